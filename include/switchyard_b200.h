@@ -29,6 +29,7 @@ extern "C" {
 
 #define SY_DTYPE_F16 0
 #define SY_DTYPE_BF16 1
+#define SY_DTYPE_F32 2 /* rows and weights of the row operators and the quantisers only */
 
 /* Message of the calling thread's last failing call ("" if none). Never NULL. */
 const char* sy_last_error(void);
@@ -65,7 +66,8 @@ size_t sy_sort_scratch_bytes(int m, int n_experts);
 /* sort_by_expert — replaces `sort_by_expert` (moe_kernels.cu:142-157, kernels l.94-139 and the
  * torch cumsum between them). Stable counting sort of the flat choice list (i = token*top_k +
  * slot) by expert id, no atomics, same result every run.
- * idx int32 [m] (m = n_tokens*top_k, values in [0, n_experts)), w 16-bit [m].
+ * idx int32 [m] (m = n_tokens*top_k, values in [0, n_experts)), w 16-bit [m] (or NULL: no weights,
+ * wsorted is not written).
  * Outputs: counts int32 [n_experts]; offsets int32 [n_experts+1] (exclusive prefix);
  * token int32 [m] (= i / top_k of the choice in that sorted row); wsorted 16-bit [m];
  * pos_of int32 [m] (sorted row of choice i). m == 0 zero-fills counts and offsets.
@@ -229,11 +231,69 @@ int sy_gather_rows(const void* src, const int32_t* index, int n, int row_bytes, 
  * two device buffers (same GPU or peers) on `stream`. */
 int sy_copy_async(void* dst, const void* src, size_t bytes, void* stream);
 
-
 /* enable_peer_access — replaces `enable_peer_access` (moe_kernels.cu:477-489). Sets
  * *enabled_out to 1 if `device` can (now) address `peer`'s memory, 0 if the hardware cannot.
  * Already-enabled is not an error. */
 int sy_enable_peer_access(int device, int peer, int* enabled_out);
+
+/* ---- rows into expert order and back, with their gradients ------------------------------------
+ * No counterpart in the reference (inference only). Rows are f16, bf16 or f32, a multiple of
+ * 16 bytes each and 16-byte aligned; top_k <= 8; pos_of int32 [n_tokens, top_k] and offsets int32
+ * [n_experts + 1] as sy_sort_by_expert gives them. A choice whose pos_of is outside
+ * [0, n_tokens * top_k) has no row: it is skipped, its weight's gradient is 0. Rows from
+ * offsets[n_experts] on (as many as choices were skipped) are set to zero. */
+
+/* permute_rows — x[pos_of[t, j], :] = h[t, :], x [n_tokens * top_k, hidden]. */
+int sy_permute_rows(const void* h, const int32_t* pos_of, const int32_t* offsets, int n_tokens, int top_k, int n_experts,
+                    int hidden, int dtype, void* x, void* stream);
+
+/* unpermute_rows — out[t, :] = sum_j w[t, j] * y[pos_of[t, j], :], summed in float32 in ascending
+ * row (sy_combine's order: expert id, ties by slot), rounded once. w [n_tokens, top_k] in the
+ * rows' type or f32 (w_dtype); NULL: all one. With w NULL it is the gradient of sy_permute_rows. */
+int sy_unpermute_rows(const void* y, const void* w, int w_dtype, const int32_t* pos_of, int n_tokens, int top_k, int hidden,
+                      int dtype, void* out, void* stream);
+
+/* unpermute_rows_grad — the gradients of sy_unpermute_rows in one pass over dout and y:
+ * dy[pos_of[t, j], :] = w[t, j] * dout[t, :];  dw[t, j] = sum_h dout[t, h] * y[pos_of[t, j], h]
+ * (float32, a fixed order, rounded once to w_dtype). Either of dy, dw may be NULL; y is read for
+ * dw only. */
+int sy_unpermute_rows_grad(const void* dout, const void* y, const void* w, int w_dtype, const int32_t* pos_of,
+                           const int32_t* offsets, int n_tokens, int top_k, int n_experts, int hidden, int dtype, void* dy,
+                           void* dw, void* stream);
+
+/* ---- experts in 8-bit floats --------------------------------------------------------------------
+ * No counterpart in the reference. e4m3 values with a float32 scale for each block: 1 x 128 for
+ * rows, 128 x 128 for weights. With m = max(largest magnitude of the block, 2^-96):
+ * scale = m / 448, q = e4m3(448 x / m), a correctly rounded division and then the nearest e4m3
+ * value, ties to even. A NaN or infinity makes its block's scale NaN or infinite. */
+
+/* quantize_rows — x [n_tokens, hidden] f16, bf16 or f32 into q uint8 [rows, hidden] and scale f32
+ * [ceil(hidden / 128), rows] (block-major: a block's scales of consecutive rows are contiguous).
+ * pos_of NULL (top_k 1): row t stays row t, rows = n_tokens. Otherwise row t goes to its top_k
+ * places in expert order as in sy_permute_rows, rows = n_tokens * top_k; rows without a choice get
+ * zero values and zero scales. hidden % 16 == 0, x and q 16-byte aligned. */
+int sy_quantize_rows(const void* x, const int32_t* pos_of, const int32_t* offsets, int n_tokens, int top_k, int n_experts,
+                     int hidden, int dtype, void* q, float* scale, void* stream);
+
+/* quantize_weight — w [n_mats, n_rows, k_dim] into q of the same shape and scale f32
+ * [n_mats, ceil(n_rows / 128), ceil(k_dim / 128)]. A gate_up stack [E, 2*I, H] is quantised as 2*E
+ * matrices of I rows, so that no block holds gate and up rows. k_dim % 16 == 0. */
+int sy_quantize_weight(const void* w, int n_mats, int n_rows, int k_dim, int dtype, void* q, float* scale, void* stream);
+
+/* grouped_gemm_fp8 — sy_grouped_gemm on 8-bit operands: for row r of expert e
+ *   C[r, n] = round16( scale[r] * sum_b x_scale[b, r] * w_scale[e, n / 128, b] * <x[r, block b], w[e, n, block b]> )
+ * x uint8 [rows, k_dim] and x_scale as sy_quantize_rows writes them; w uint8 [n_experts, n_full,
+ * k_dim], w_scale [n_experts, blocks, ceil(k_dim / 128)]. swiglu: n_full = 2*n_out, gate rows then
+ * up rows, blocks = 2 * ceil(n_out / 128) (each half's on its own), C = round16(silu(gate) * up).
+ * Sums, scales and epilogue in float32, ONE rounding. scale 16-bit [rows] or NULL (not with swiglu).
+ * offsets int32 [n_experts + 1]; values outside [0, rows] are clamped, rows of no expert are set to
+ * zero. A row's bits do not depend on the other rows of its expert or on the tile.
+ * tile: 0 = chosen from the mean rows per expert; 1 = 128 rows x 128 weight rows, 2 = 128 x 256,
+ * 3 = 256 x 256 over a pair of CTAs. k_dim % 16 == 0, n_out % 8 == 0, n_experts <= 256, x, w and C
+ * 16-byte aligned. */
+int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const void* w, const float* w_scale, const int32_t* offsets,
+                        int n_experts, int rows, int n_out, int k_dim, int swiglu, const void* scale, void* C, int dtype,
+                        int tile, void* stream);
 
 /* ---- expert parallelism over device-driven transport ----------------------------------------
  * The entry points below have no single counterpart in the reference: together they replace

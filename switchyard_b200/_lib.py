@@ -13,7 +13,7 @@ from ctypes import c_char_p, c_int, c_size_t, c_void_p
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libswitchyard_b200.so")
 
-SY_DTYPE_F16, SY_DTYPE_BF16 = 0, 1
+SY_DTYPE_F16, SY_DTYPE_BF16, SY_DTYPE_F32 = 0, 1, 2
 SY_ERR_DEVICE = -3
 
 # name -> (restype, argtypes); must list every symbol the header declares
@@ -52,6 +52,15 @@ SYMBOLS = {
     "sy_gather_rows": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "sy_copy_async": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "sy_enable_peer_access": (c_int, [c_int, c_int, ctypes.POINTER(c_int)]),
+    "sy_permute_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "sy_unpermute_rows": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "sy_unpermute_rows_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                       c_int, c_void_p, c_void_p, c_void_p]),
+    "sy_quantize_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                 c_void_p]),
+    "sy_quantize_weight": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "sy_grouped_gemm_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                    c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "sy_grouped_segments": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                     c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "sy_ep_dispatch_scratch_bytes": (c_size_t, [c_int]),

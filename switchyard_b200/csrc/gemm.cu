@@ -44,6 +44,7 @@
 
 #include "common.cuh"
 #include "ep_push.cuh"
+#include "tensor_map.cuh"
 
 namespace sy {
 
@@ -1033,37 +1034,26 @@ static int encode_fn(EncodeTiledFn* out) {
   return SY_OK;
 }
 
-// Tensor map over the stacked expert weights as a [rows, K] matrix; box = box_rows x 64 k.
-static int weight_map(CUtensorMap* map, const void* B, uint64_t rows, uint64_t K, int dtype, int box_rows) {
+int tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base, uint64_t rows, uint64_t cols,
+                  int box_rows, int box_cols) {
   EncodeTiledFn encode;
   int rc = encode_fn(&encode);
   if (rc != SY_OK) return rc;
-  cuuint64_t dims[2] = {K, rows};
-  cuuint64_t strides[1] = {K * 2};
-  cuuint32_t box[2] = {GM_ATOM_K, (cuuint32_t)box_rows};
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {cols * elem_bytes};
+  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   cuuint32_t elem[2] = {1, 1};
-  CUresult r = encode(map, dtype == SY_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                      2, const_cast<void*>(B), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(SY_ERR_CUDA, "grouped kernel: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return SY_OK;
 }
 
-// Tensor map over activations whose rows are the ranges' rows themselves, as a [rows, K]
-// matrix; box = box_rows x 64 k.
-static int activation_map(CUtensorMap* map, const void* A, uint64_t rows, uint64_t K, int dtype, int box_rows) {
-  EncodeTiledFn encode;
-  int rc = encode_fn(&encode);
-  if (rc != SY_OK) return rc;
-  cuuint64_t dims[2] = {K, rows};
-  cuuint64_t strides[1] = {K * 2};
-  cuuint32_t box[2] = {GM_ATOM_K, (cuuint32_t)box_rows};
-  cuuint32_t elem[2] = {1, 1};
-  CUresult r = encode(map, dtype == SY_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                      2, const_cast<void*>(A), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(SY_ERR_CUDA, "grouped kernel: cuTensorMapEncodeTiled (activations) failed (%d)", (int)r);
-  return SY_OK;
+// Tensor map over the stacked expert weights, or over activations whose rows are the ranges' rows
+// themselves, as a [rows, K] matrix; box = box_rows x 64 k.
+static int matrix_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, int dtype, int box_rows) {
+  return tensor_map_2d(map, dtype == SY_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base,
+                       rows, K, box_rows, GM_ATOM_K);
 }
 
 // One contraction as the entry points describe it.
@@ -1150,12 +1140,12 @@ static int launch_gemm(const GroupedArgs& a) {
   k.weight_div = weight_div;
   for (int i = 0; i < a.n_problems; ++i) {
     const ProblemDesc& d = a.p[i];
-    rc = weight_map(&k.p[i].map, d.B, (uint64_t)experts * (d.swiglu ? 2 : 1) * d.n_out, (uint64_t)d.k_dim, a.dtype,
+    rc = matrix_map(&k.p[i].map, d.B, (uint64_t)experts * (d.swiglu ? 2 : 1) * d.n_out, (uint64_t)d.k_dim, a.dtype,
                     Shape<SH>::BOX_ROWS);
     if (rc != SY_OK) return rc;
     k.p[i].x_tma = !d.a_rows && a.group_div == 1 && a.rows > 0;
     if (k.p[i].x_tma) {
-      rc = activation_map(&k.p[i].xmap, d.A, (uint64_t)a.rows, (uint64_t)d.k_dim, a.dtype, Shape<SH>::XR);
+      rc = matrix_map(&k.p[i].xmap, d.A, (uint64_t)a.rows, (uint64_t)d.k_dim, a.dtype, Shape<SH>::XR);
       if (rc != SY_OK) return rc;
     }
     k.p[i].A = d.A;

@@ -117,7 +117,7 @@ __device__ __forceinline__ void scatter_chunk(const int* idx, const T* w, int m,
     __syncwarp();
     if (ok) {
       token[pos] = i / k;
-      wsorted[pos] = COHERENT ? ldcg16(w + i) : w[i];
+      if (w) wsorted[pos] = COHERENT ? ldcg16(w + i) : w[i];  // w absent: a plan without weights
       pos_of[i] = pos;
     }
   }
@@ -401,7 +401,7 @@ extern "C" int sy_sort_by_expert(const int32_t* idx, const void* w, int m, int t
     SY_CUDA(cudaMemsetAsync(offsets, 0, sizeof(int32_t) * (n_experts + 1), s));
     return SY_OK;
   }
-  SY_REQUIRE(idx && w && token && wsorted && pos_of, "sort_by_expert: null pointer");
+  SY_REQUIRE(idx && token && (wsorted || !w) && pos_of, "sort_by_expert: null pointer");
   size_t need = sy_sort_scratch_bytes(m, n_experts);
   SY_REQUIRE(need == 0 || (scratch && scratch_bytes >= need), "sort_by_expert: %zu bytes of scratch needed, %zu given",
              need, scratch_bytes);

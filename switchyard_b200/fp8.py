@@ -1,0 +1,95 @@
+"""Experts in 8-bit floats: e4m3 values with a float32 scale for each block of 128 (1 x 128 for rows,
+128 x 128 for weights), quantised by csrc/quant8.cu and multiplied by csrc/gemm_fp8.cu. Half the bytes
+of the 16-bit experts where decode reads weights, twice the tensor-core rate where prefill
+multiplies. Beyond the reference, which has 16-bit experts only.
+
+    gate_up8 = fp8.quantize_weight(gate_up, halves=2)     # [E, 2*I, H], once at load
+    down8 = fp8.quantize_weight(down)                      # [E, H, I]
+    out = kernels.moe_layer(h, router, gate_up8, down8, top_k, norm)
+
+For inference: no call here has a gradient, and an input that requires one is refused while
+gradients are recorded. Everything is enqueued on the current stream; nothing synchronises."""
+
+from typing import NamedTuple
+
+import torch
+
+from . import rows as _rows
+
+
+class Rows8(NamedTuple):
+    """q float8_e4m3fn [rows, K], scale float32 [ceil(K/128), rows]: row r, column c stands for
+    q[r, c] * scale[c // 128, r]."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    def dequantize(self, dtype=torch.float32):
+        K = self.q.shape[1]
+        return (self.q.float() * self.scale.t().repeat_interleave(128, 1)[:, :K]).to(dtype)
+
+
+class Weight8(NamedTuple):
+    """q float8_e4m3fn [E, N, K], scale float32 [E, halves * ceil(N/halves/128), ceil(K/128)] for blocks
+    of 128 x 128; a gate_up stack counts its blocks in each half on its own (halves 2), which
+    is the plain layout when the halves are multiples of 128."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def dequantize(self, dtype=torch.float32, halves=1):
+        E, N, K = self.q.shape
+        s = self.scale.reshape(E * halves, -1, self.scale.shape[-1])
+        s = s.repeat_interleave(128, 1)[:, :N // halves].repeat_interleave(128, 2)[:, :, :K]
+        return (self.q.float() * s.reshape(E, N, K)).to(dtype)
+
+
+def _no_grad(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
+
+
+def quantize_rows(x, plan=None):
+    """Rows8 of x [N, H] (fp16, bf16 or fp32, H a multiple of 16). With a rows.SortPlan the rows come in
+    expert order (as rows.permute_rows brings them), each token quantised once. With m the largest
+    magnitude of a block, at least 2^-96: scale = m / 448, q = e4m3(448 x / m), correctly rounded.
+    A NaN or infinity in a block makes its scale NaN or infinite."""
+    _no_grad("quantize_rows", x)
+    x = x.contiguous()
+    if plan is None:
+        return Rows8(*_rows._ext().quantize_rows(x))
+    return Rows8(*_rows._ext().quantize_rows(x, plan.pos_of, plan.offsets))
+
+
+def quantize_weight(w, halves=1):
+    """Weight8 of w [E, N, K] (fp16, bf16 or fp32, K a multiple of 16). halves=2 for a gate_up stack."""
+    _no_grad("quantize_weight", w)
+    return Weight8(*_rows._ext().quantize_weight(w.contiguous(), halves))
+
+
+def grouped_gemm(x, w, offsets, swiglu=False, scale=None, dtype=torch.bfloat16):
+    """Every expert's rows times its weights: x Rows8 in expert order, w Weight8, offsets int32 [E+1].
+    C [rows, N] = x w^T; with scale [rows] (dtype) every row times its own; with swiglu (w quantised
+    in two halves) C [rows, N/2] = silu(x gate^T) * (x up^T). Float32 up to the one rounding to `dtype`
+    (bf16 or fp16). Rows of no expert are zero. A row's bits depend on nothing but the row and its
+    expert's weights."""
+    _no_grad("grouped_gemm", scale)
+    return _rows._ext().grouped_gemm_fp8(x.q, x.scale, w.q, w.scale, offsets, swiglu, scale, dtype)
+
+
+def sorted_experts(h, plan, wsorted, gate_up, down, mode="auto"):
+    """The expert FFN on 8-bit weights for a sorted batch: rows quantised into expert order, gate/up
+    product with SwiGLU, its result quantised, down product times the router weights wsorted.
+    Returns y [N*k, H] in h's dtype, for combine. `mode` is checked and otherwise without effect."""
+    if mode not in ("auto", "gemv", "gemm", "cublas"):
+        raise RuntimeError(f"sorted_experts: unknown mode {mode!r}")
+    if not (isinstance(gate_up, Weight8) and isinstance(down, Weight8)):
+        raise RuntimeError("sorted_experts: gate_up and down must both be 8-bit (fp8.Weight8) or both 16-bit")
+    act = grouped_gemm(quantize_rows(h, plan), gate_up, plan.offsets, swiglu=True, dtype=h.dtype)
+    return grouped_gemm(quantize_rows(act), down, plan.offsets, scale=wsorted, dtype=h.dtype)

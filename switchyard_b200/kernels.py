@@ -15,6 +15,9 @@ Differences a caller can observe:
   * there is no cuBLAS mode; "cublas" is accepted as an alias of "gemm";
   * `experts(mode="auto")` chooses from the token count, not from a device-to-host read of
     the largest expert's row count, so the layer never synchronises;
+  * `experts`, `moe_layer` and `GraphedLayer` also take 8-bit expert weights (`fp8.Weight8` for both
+    gate_up and down): the rows are then quantised on their way into expert order and both
+    products run in e4m3, whatever `mode` says (the tile follows the batch, the bits do not);
   * `route_fused` computes the router logits inside the routing launch instead of calling the
     library GEMM. It is not what `moe_layer` uses unless SWITCHYARD_FUSED_ROUTER=1 (or
     `route_and_sort(..., fused=True)`): measured on a B200 the library GEMM followed by the
@@ -31,7 +34,7 @@ import ctypes
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, fp8, rows
 
 _EXT = None
 
@@ -44,10 +47,39 @@ def _dtype_code(t, what):
     raise RuntimeError(f"{what}: fp16 or bf16 expected, got {t.dtype}")
 
 
+def _row_code(t, what):
+    """Type code of rows and weights that may also be fp32."""
+    return _lib.SY_DTYPE_F32 if t.dtype == torch.float32 else _dtype_code(t, what)
+
+
 def _check(t, name):
     if not (t.is_cuda and t.is_contiguous()):
         raise RuntimeError(f"{name} must be a contiguous CUDA tensor")
     return t
+
+
+def _check_places(pos_of, offsets, like, name):
+    """(tokens, top_k) of a plan's tensors, which must be on the rows' device."""
+    if pos_of.dim() != 2 or pos_of.dtype != torch.int32 or pos_of.device != like.device:
+        raise RuntimeError(f"{name}: pos_of must be int32 [tokens, top_k] on the rows' device")
+    _check(pos_of, "pos_of")
+    if offsets is not None:
+        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.device != like.device:
+            raise RuntimeError(f"{name}: offsets must be int32 [experts + 1] on the rows' device")
+        _check(offsets, "offsets")
+    return pos_of.shape
+
+
+def _check_weighted(y, w, N, k, name):
+    """Type codes of y [N*k, H] and its weights [N, k] (None: the rows' code)."""
+    code = _row_code(_check(y, "y"), name)
+    if y.dim() != 2 or y.shape[0] != N * k:
+        raise RuntimeError(f"{name}: y must be [{N * k}, hidden], got {list(y.shape)}")
+    if w is None:
+        return code, code
+    if w.shape != (N, k) or w.dtype not in (y.dtype, torch.float32) or w.device != y.device:
+        raise RuntimeError(f"{name}: w must be [{N}, {k}], float32 or of the rows' dtype, on their device")
+    return code, _row_code(_check(w, "w"), name)
 
 
 def _ptr(t):
@@ -203,17 +235,18 @@ class Ext:
         return [idx, w]
 
     def sort_by_expert(self, idx, w, E):
-        _check(idx, "idx"), _check(w, "w")
+        """w may be None (a plan without weights): wsorted is then None."""
+        _check(idx, "idx")
         if idx.dtype != torch.int32:
             raise RuntimeError("sort_by_expert: idx must be int32")
         M = idx.numel()
         k = idx.shape[1] if idx.dim() == 2 else 1
-        code = _dtype_code(w, "sort_by_expert")
+        code = _dtype_code(_check(w, "w"), "sort_by_expert") if w is not None else _lib.SY_DTYPE_F16
         dev = idx.device
         ints = torch.empty(2 * E + 1 + 2 * M, dtype=torch.int32, device=dev)
         counts, offsets = ints[:E], ints[E:2 * E + 1]
         token, pos_of = ints[2 * E + 1:2 * E + 1 + M], ints[2 * E + 1 + M:]
-        wsorted = torch.empty(M, dtype=w.dtype, device=dev)
+        wsorted = torch.empty(M, dtype=w.dtype, device=dev) if w is not None else None
         need = self.lib.sy_sort_scratch_bytes(M, int(E))
         scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         with _Device(dev) as stream:
@@ -294,6 +327,122 @@ class Ext:
                                              _ptr(out), code, stream)
             _lib.check(rc, "combine")
         return out
+
+    def permute_rows(self, h, pos_of, offsets):
+        """x [N*k, H] with x[pos_of[t, j]] = h[t] (rows.permute_rows adds the gradient)."""
+        N, k = _check_places(pos_of, offsets, h, "permute_rows")
+        if h.dim() != 2 or h.shape[0] != N:
+            raise RuntimeError(f"permute_rows: h must be [{N}, hidden], got {list(h.shape)}")
+        code, H = _row_code(_check(h, "h"), "permute_rows"), h.shape[1]
+        x = torch.empty(N * k, H, dtype=h.dtype, device=h.device)
+        with _Device(h.device) as stream:
+            _lib.check(self.lib.sy_permute_rows(_ptr(h), _ptr(pos_of), _ptr(offsets), N, k, offsets.numel() - 1, H, code,
+                                                _ptr(x), stream), "permute_rows")
+        return x
+
+    def unpermute_rows(self, y, w, pos_of):
+        """out [N, H] = sum_j w[t, j] * y[pos_of[t, j]]; w None: all one (rows.unpermute_rows adds
+        the gradients)."""
+        N, k = _check_places(pos_of, None, y, "unpermute_rows")
+        code, wcode = _check_weighted(y, w, N, k, "unpermute_rows")
+        H = y.shape[1]
+        out = torch.empty(N, H, dtype=y.dtype, device=y.device)
+        with _Device(y.device) as stream:
+            _lib.check(self.lib.sy_unpermute_rows(_ptr(y), _ptr(w), wcode, _ptr(pos_of), N, k, H, code, _ptr(out), stream),
+                       "unpermute_rows")
+        return out
+
+    def unpermute_rows_grad(self, dout, y, w, pos_of, offsets, need_dy=True, need_dw=True):
+        """(dy, dw) of unpermute_rows; what is not needed is None, and y may be None without dw."""
+        N, k = _check_places(pos_of, offsets, dout, "unpermute_rows_grad")
+        code, H = _row_code(_check(dout, "dout"), "unpermute_rows_grad"), dout.shape[1]
+        if dout.shape != (N, H):
+            raise RuntimeError(f"unpermute_rows_grad: dout must be [{N}, hidden], got {list(dout.shape)}")
+        if y is not None and (y.dtype != dout.dtype or y.shape != (N * k, H) or y.device != dout.device):
+            raise RuntimeError(f"unpermute_rows_grad: y must be [{N * k}, {H}] in dout's dtype and on its device")
+        if need_dw and (y is None or w is None):
+            raise RuntimeError("unpermute_rows_grad: the weights' gradient needs y and w")
+        wcode = code
+        if y is not None:
+            _check(y, "y")
+        if w is not None:
+            if w.shape != (N, k) or w.dtype not in (dout.dtype, torch.float32) or w.device != dout.device:
+                raise RuntimeError(f"unpermute_rows_grad: w must be [{N}, {k}], float32 or of the rows' dtype")
+            wcode = _row_code(_check(w, "w"), "unpermute_rows_grad")
+        dy = torch.empty(N * k, H, dtype=dout.dtype, device=dout.device) if need_dy else None
+        dw = torch.empty_like(w) if need_dw else None
+        with _Device(dout.device) as stream:
+            _lib.check(self.lib.sy_unpermute_rows_grad(_ptr(dout), _ptr(y), _ptr(w), wcode, _ptr(pos_of), _ptr(offsets), N, k,
+                                                       offsets.numel() - 1, H, code, _ptr(dy), _ptr(dw), stream),
+                       "unpermute_rows_grad")
+        return dy, dw
+
+    def quantize_rows(self, x, pos_of=None, offsets=None):
+        """(q float8_e4m3fn [rows, H], scale float32 [ceil(H/128), rows]) of x [N, H]; with pos_of and
+        offsets the rows come in expert order, rows = N*k."""
+        if x.dim() != 2:
+            raise RuntimeError(f"quantize_rows: x must be [tokens, hidden], got {list(x.shape)}")
+        N, H = x.shape
+        k = 1
+        code = _row_code(_check(x, "x"), "quantize_rows")
+        if pos_of is not None:
+            n, k = _check_places(pos_of, offsets, x, "quantize_rows")
+            if n != N:
+                raise RuntimeError(f"quantize_rows: x has {N} rows, the plan {n} tokens")
+        q = torch.empty(N * k, H, dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty((H + 127) // 128, N * k, dtype=torch.float32, device=x.device)
+        with _Device(x.device) as stream:
+            _lib.check(self.lib.sy_quantize_rows(_ptr(x), _ptr(pos_of), _ptr(offsets), N, k,
+                                                 offsets.numel() - 1 if pos_of is not None else 0, H, code, _ptr(q),
+                                                 _ptr(scale), stream), "quantize_rows")
+        return q, scale
+
+    def quantize_weight(self, w, halves=1):
+        """(q float8_e4m3fn [E, N, K], scale float32 [E, halves * ceil(N/halves/128), ceil(K/128)])."""
+        if w.dim() != 3 or halves not in (1, 2) or w.shape[1] % halves:
+            raise RuntimeError(f"quantize_weight: w must be [experts, rows, k] with rows in {halves} equal parts "
+                               f"(1 or 2), got {list(w.shape)}")
+        code = _row_code(_check(w, "w"), "quantize_weight")
+        E, N, K = w.shape
+        q = torch.empty(E, N, K, dtype=torch.float8_e4m3fn, device=w.device)
+        scale = torch.empty(E, halves * ((N // halves + 127) // 128), (K + 127) // 128, dtype=torch.float32, device=w.device)
+        with _Device(w.device) as stream:
+            _lib.check(self.lib.sy_quantize_weight(_ptr(w), E * halves, N // halves, K, code, _ptr(q), _ptr(scale), stream),
+                       "quantize_weight")
+        return q, scale
+
+    def grouped_gemm_fp8(self, x, x_scale, w, w_scale, offsets, swiglu, scale, dtype, tile=0):
+        """The experts' product of 8-bit rows and weights (sy_grouped_gemm_fp8): C [rows, n_out]."""
+        name = "grouped_gemm_fp8"
+        for t, what, dt, dims in ((x, "x", torch.float8_e4m3fn, 2), (x_scale, "x_scale", torch.float32, 2),
+                                  (w, "w", torch.float8_e4m3fn, 3), (w_scale, "w_scale", torch.float32, 3),
+                                  (offsets, "offsets", torch.int32, 1)):
+            if t.dtype != dt or t.dim() != dims or t.device != x.device:
+                raise RuntimeError(f"{name}: {what} must be {dt} with {dims} dimensions, on x's device")
+            _check(t, what)
+        (rows, K), (E, Nfull, wk) = x.shape, w.shape
+        parts = 2 if swiglu else 1
+        if Nfull % parts:
+            raise RuntimeError(f"{name}: swiglu needs gate and up rows, got {Nfull} weight rows")
+        n_out, kb = Nfull // parts, (K + 127) // 128
+        if wk != K or x_scale.shape != (kb, rows) or offsets.numel() != E + 1:
+            raise RuntimeError(f"{name}: x [{rows}, {K}] needs x_scale [{kb}, {rows}], weights of k {K} and offsets [{E + 1}]")
+        if w_scale.shape != (E, parts * ((n_out + 127) // 128), kb):
+            raise RuntimeError(f"{name}: w_scale must be [{E}, {parts * ((n_out + 127) // 128)}, {kb}], got "
+                               f"{list(w_scale.shape)}" + (" (quantise gate and up as two halves)" if swiglu else ""))
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError(f"{name}: the result is fp16 or bf16, not {dtype}")
+        if scale is not None and (scale.dtype != dtype or scale.shape != (rows,) or scale.device != x.device):
+            raise RuntimeError(f"{name}: scale must be [{rows}] in the result's dtype")
+        C = torch.empty(rows, n_out, dtype=dtype, device=x.device)
+        code = _lib.SY_DTYPE_F16 if dtype == torch.float16 else _lib.SY_DTYPE_BF16
+        if scale is not None:
+            _check(scale, "scale")
+        with _Device(x.device) as stream:
+            _lib.check(self.lib.sy_grouped_gemm_fp8(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(offsets), E, rows,
+                                                    n_out, K, int(bool(swiglu)), _ptr(scale), _ptr(C), code, int(tile),
+                                                    stream), name)
+        return C
 
     def gather_rows(self, src, index, dst):
         _check(src, "src"), _check(index, "index"), _check(dst, "dst")
@@ -394,6 +543,8 @@ def ffn(x, a_rows, offsets, counts, wsorted, gate_up, down, rows, mode, host_cou
     output scaled by its router weight, [rows, H] (switchyard/kernels.py:48-73). `counts` and
     `host_counts` are accepted for compatibility; neither kernel needs them."""
     E = ext()
+    if isinstance(gate_up, fp8.Weight8) or isinstance(down, fp8.Weight8):
+        raise RuntimeError("ffn: 8-bit experts run through experts() and moe_layer(), or fp8.grouped_gemm")
     if rows == 0:
         return torch.empty(0, down.shape[1], dtype=x.dtype, device=x.device)
     x = x.contiguous()
@@ -418,6 +569,9 @@ def _sorted_experts(h, srt, gate_up, down, top_k, mode, scratch=None, residual=N
     """From sorted choices (idx, w, counts, offsets, token, wsorted, pos_of) to the layer's output
     (plus the residual, when given)."""
     idx, _, counts, offsets, token, wsorted, pos_of = srt
+    if isinstance(gate_up, fp8.Weight8) or isinstance(down, fp8.Weight8):
+        y = fp8.sorted_experts(h, rows.SortPlan(counts, offsets, token, pos_of.view(idx.shape)), wsorted, gate_up, down, mode)
+        return ext().combine(y, pos_of, idx, h.shape[0], residual)
     if mode == "auto":
         mode = auto_mode(idx.numel(), gate_up.shape[0])  # no device-to-host read
     if mode == "gemv" and 0 < top_k <= 8 and idx.numel() >= FUSED_COMBINE_MIN_ROWS:

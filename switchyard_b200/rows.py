@@ -1,0 +1,88 @@
+"""Token rows into expert order and back, for code that brings its own experts and for training:
+both directions have gradients. The sort itself is `kernels`' (`sort_by_expert`), the kernels are in
+csrc/rows.cu. Beyond the reference, which infers only.
+
+    plan = rows.plan(idx, n_experts)              # idx [N, k]: every token's experts
+    x = rows.permute_rows(h, plan)                # [N*k, H], expert e owns plan.offsets[e]:plan.offsets[e+1]
+    y = my_experts(x, plan.offsets)
+    out = rows.unpermute_rows(y, w, plan)         # [N, H]: every token's rows, weighted and summed
+
+Rows are fp16, bf16 or fp32 with a row of a multiple of 16 bytes, top_k is at most 8. Everything is
+enqueued on the current stream; nothing synchronises, and a plan's addresses are all that a
+captured graph keeps. RuntimeError on any other argument."""
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+
+class SortPlan(NamedTuple):
+    """Where every choice's row goes. pos_of[t, j] is the sorted row of token t's j-th choice, -1
+    where its expert id is outside [0, experts): such a choice has no row, and as many rows at
+    the end belong to none (permute_rows sets them to zero)."""
+    counts: torch.Tensor   # int32 [experts] rows per expert
+    offsets: torch.Tensor  # int32 [experts + 1] exclusive prefix of counts
+    token: torch.Tensor    # int32 [N*k] token of each sorted row (undefined from offsets[experts] on)
+    pos_of: torch.Tensor   # int32 [N, k]
+
+
+def _ext():
+    from . import kernels
+    return kernels.ext()
+
+
+def plan(idx, n_experts):
+    """The plan of idx [N, k] (any integer type): a stable sort of the choices by expert."""
+    if idx.dim() != 2:
+        raise RuntimeError(f"plan: idx must be [tokens, top_k], got {list(idx.shape)}")
+    counts, offsets, token, _, pos_of = _ext().sort_by_expert(idx.to(torch.int32).contiguous(), None, n_experts)
+    return SortPlan(counts, offsets, token, pos_of.view(idx.shape))
+
+
+class _Permute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, offsets, pos_of):
+        ctx.save_for_backward(pos_of)
+        return _ext().permute_rows(h, pos_of, offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dx):
+        pos_of, = ctx.saved_tensors
+        return _ext().unpermute_rows(dx.contiguous(), None, pos_of), None, None
+
+
+class _Unpermute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, w, offsets, pos_of):
+        ctx.save_for_backward(y if w is not None and ctx.needs_input_grad[1] else None, w, offsets, pos_of)
+        return _ext().unpermute_rows(y, w, pos_of)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        y, w, offsets, pos_of = ctx.saved_tensors
+        need_dy, need_dw = ctx.needs_input_grad[:2]
+        dy, dw = _ext().unpermute_rows_grad(dout.contiguous(), y, w, pos_of, offsets, need_dy, need_dw)
+        return dy, dw, None, None
+
+
+def permute_rows(h, plan):
+    """x [N*k, H]: row plan.pos_of[t, j] is h[t]. Gradient: every token's rows of dx summed in float32
+    in ascending row, rounded once."""
+    h = h.contiguous()
+    if torch.is_grad_enabled() and h.requires_grad:
+        return _Permute.apply(h, plan.offsets, plan.pos_of)
+    return _ext().permute_rows(h, plan.pos_of, plan.offsets)
+
+
+def unpermute_rows(y, w, plan):
+    """out [N, H]: sum over j of w[t, j] * y[plan.pos_of[t, j]], in float32 in ascending row (the order of
+    `combine`), rounded once. w [N, k] in y's dtype or float32, or None for a plain sum. Gradients:
+    dy (rows of no choice: zero) and dw, the dot products in float32."""
+    y = y.contiguous()
+    w = w.contiguous() if w is not None else None
+    if torch.is_grad_enabled() and (y.requires_grad or (w is not None and w.requires_grad)):
+        return _Unpermute.apply(y, w, plan.offsets, plan.pos_of)
+    return _ext().unpermute_rows(y, w, plan.pos_of)

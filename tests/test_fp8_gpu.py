@@ -1,0 +1,289 @@
+"""The e4m3 quantisers and the experts' 8-bit product (switchyard_b200.fp8) against plain 64-bit
+forms. The quantisers are exact: the same e4m3 values, the same float32 scales. The product's
+bounds are derived in rows_fp8_cases (product_bound, swiglu_bound)."""
+
+import pytest
+import torch
+
+import rows_fp8_cases as rc
+from rows_fp8_cases import places, product64, product_bound, quantize64, rounding, swiglu_bound
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def Q():
+    from switchyard_b200 import fp8, kernels
+    kernels.ext()
+    yield fp8
+    assert kernels.ext().device_status(DEV) == 0
+
+
+def same(a, b):
+    """Equal, NaN where NaN."""
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a[~a.isnan()], b[~b.isnan()])
+
+
+def same_bits(a, b):
+    return a.dtype == b.dtype and torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def hard_rows(N, H, dtype, seed):
+    """Rows with the values that a quantiser can get wrong: zeros, the type's ends, subnormals, one
+    large value among small ones, values midway between two e4m3 values, infinities, NaN."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(N, H, generator=g) * torch.exp(3 * torch.randn(N, 1, generator=g))
+    x = x.to(dtype)
+    info = torch.finfo(dtype)
+    x[0] = 0
+    if N > 1:
+        x[1, : min(H, 64)] = info.max
+        x[1, min(H, 64):] = -info.max
+    if N > 2:
+        x[2] = info.smallest_normal / 2
+    if N > 3:
+        x[3] *= 1e-3
+        x[3, 0] = info.max / 2
+    if N > 4:
+        x[4] = torch.arange(H).to(dtype) % 17 / 16
+        x[4, 0] = 1.75  # 448 / 256: quotients of sixteenths lie midway between e4m3 values
+    if N > 5:
+        x[5, 1] = float("inf")
+    if N > 6:
+        x[6, H - 1] = float("nan")
+    return x
+
+
+@pytest.mark.parametrize("N,H", [(1, 16), (1, 2048), (7, 128), (9, 144), (40, 1040), (300, 256), (8, 4112)])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_quantize_rows_is_exact(Q, N, H, dtype):
+    x = hard_rows(N, H, dtype, N + H)
+    got = Q.quantize_rows(x.to(DEV))
+    q, s = quantize64(x, 1)
+    assert got.q.dtype == torch.float8_e4m3fn and got.q.shape == (N, H) and got.scale.shape == (-(-H // 128), N)
+    assert same(got.scale.cpu().t(), s) and same(got.q.cpu().double(), q)
+
+
+@pytest.mark.parametrize("N,k,E,H,bad", [(1, 8, 64, 2048, 0), (5, 3, 8, 48, 0), (130, 8, 64, 256, 0), (33, 4, 60, 1040, 9)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantize_rows_into_expert_order(Q, N, k, E, H, bad, dtype):
+    from switchyard_b200 import kernels, rows
+    idx = rc.choices(N, k, E, N, bad)
+    offsets, pos = places(idx, E)
+    plan = rows.plan(idx.to(DEV), E)
+    assert kernels.ext().device_status(DEV) == (6 if bad else 0)
+    x = hard_rows(N, H, dtype, 3)
+    got = Q.quantize_rows(x.to(DEV), plan)
+    q, s = quantize64(x, 1)
+    want_q, want_s = torch.zeros(N * k, H, dtype=torch.float64), torch.zeros(N * k, s.shape[1])
+    for j in range(k):
+        ok = pos[:, j] >= 0
+        want_q[pos[ok, j]], want_s[pos[ok, j]] = q[ok], s[ok]
+    assert same(got.q.cpu().double(), want_q) and same(got.scale.cpu().t(), want_s)
+
+
+@pytest.mark.parametrize("E,N,K,halves", [(1, 8, 16, 1), (2, 128, 128, 1), (3, 200, 144, 2), (5, 136, 1040, 1), (2, 2048, 256, 2)])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_quantize_weight_is_exact(Q, E, N, K, halves, dtype):
+    w = torch.stack([hard_rows(N, K, dtype, 7 + e) for e in range(E)])
+    got = Q.quantize_weight(w.to(DEV), halves=halves)
+    parts = w.view(E * halves, N // halves, K)
+    each = [quantize64(p, 128) for p in parts]
+    assert same(got.q.cpu().double(), torch.stack([q for q, _ in each]).view(E, N, K))
+    assert same(got.scale.cpu(), torch.stack([s for _, s in each]).view(E, -1, got.scale.shape[2]))
+    fine = torch.randn(E, N, K, generator=torch.Generator().manual_seed(1))
+    back = Q.quantize_weight(fine.to(DEV), halves).dequantize(halves=halves).cpu()
+    # half a step of e4m3 relative to the value, or half its least subnormal (2^-10) times a scale below
+    # 6 / 448 (no value reaches 6), and the roundings of the division and of the product back
+    assert ((back - fine).abs() <= fine.abs() * (2.0 ** -4 + 2.0 ** -22) + 2.0 ** -10 * 6 / 448).all()
+
+
+def operands(counts, K, N, swiglu, seed):
+    """Rows in expert order and weights, e4m3 values and scales on the CPU."""
+    g = torch.Generator().manual_seed(seed)
+    M, E, parts = sum(counts), len(counts), 2 if swiglu else 1
+    offsets = torch.tensor([0] + counts).cumsum(0).int()
+    xq = (torch.randn(M, K, generator=g) * 100).to(torch.float8_e4m3fn)
+    wq = (torch.randn(E, parts * N, K, generator=g) * 100).to(torch.float8_e4m3fn)
+    xs = torch.rand(-(-K // 128), M, generator=g) * 0.01 + 1e-4
+    ws = torch.rand(E, parts * -(-N // 128), -(-K // 128), generator=g) * 3e-4 + 1e-5
+    return offsets, xq, xs, wq, ws
+
+
+SHAPES = [([1], 16, 8), ([3, 0, 1, 70], 128, 128), ([0, 0, 5], 144, 136), ([130, 1, 257], 272, 392), ([64] * 8, 256, 256),
+          ([0, 300, 0, 33, 1, 0], 1040, 1000), ([1] * 40, 2048, 64), ([600, 200], 512, 264)]
+
+
+@pytest.mark.parametrize("counts,K,N", SHAPES)
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("kind", ["plain", "scale", "swiglu"])
+def test_grouped_gemm(Q, counts, K, N, dtype, kind):
+    from switchyard_b200 import kernels
+    swiglu = kind == "swiglu"
+    offsets, xq, xs, wq, ws = operands(counts, K, N, swiglu, K + N)
+    M = xq.shape[0]
+    scale = (torch.rand(M, generator=torch.Generator().manual_seed(1)) * 2 - 1).to(dtype) if kind == "scale" else None
+    acc, mag = product64(xq, xs, wq, ws, offsets, swiglu, scale)
+    if swiglu:
+        ref, bound = swiglu_bound(acc, mag, K, N, dtype)
+    else:
+        ref, (_, bound) = acc, product_bound(acc, mag, K, dtype)
+    dev = [t.to(DEV) for t in (xq, xs, wq, ws, offsets)]
+    sd = scale.to(DEV) if scale is not None else None
+    got = Q.grouped_gemm(Q.Rows8(*dev[:2]), Q.Weight8(*dev[2:4]), dev[4], swiglu=swiglu, scale=sd, dtype=dtype)
+    assert got.shape == (M, N) and got.dtype == dtype
+    # (some operands drawn above 464 are NaN in e4m3: their rows and columns have to be NaN, and no others)
+    nan = ref.isnan()
+    assert torch.equal(got.cpu().isnan(), nan)
+    over = ((got.cpu().double() - ref).abs() - bound)[~nan]
+    assert (over <= 0).all(), over.max()
+    for tile in (1, 2, 3):  # every tile gives the same bits
+        again = kernels.ext().grouped_gemm_fp8(*dev, swiglu, sd, dtype, tile)
+        assert torch.equal(again.isnan(), got.isnan()) and torch.equal(again[~nan], got[~nan]), tile
+
+
+def test_a_rows_bits_do_not_depend_on_its_expert_s_other_rows(Q):
+    from switchyard_b200 import kernels
+    offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([200], 384, 160, False, 3))
+    full = kernels.ext().grouped_gemm_fp8(xq, xs, wq, ws, offsets, False, None, BF)
+    for at in ([7], [199, 0, 64], list(range(30, 160))):
+        sub = torch.tensor([0, len(at)], dtype=torch.int32, device=DEV)
+        got = kernels.ext().grouped_gemm_fp8(xq.view(torch.uint8)[at].view(xq.dtype), xs[:, at].contiguous(), wq, ws, sub, False,
+                                             None, BF)
+        assert same_bits(got, full[at])
+
+
+def test_rows_of_no_expert_are_zero_and_offsets_are_kept_inside(Q):
+    _, xq, xs, wq, ws = (t.to(DEV) for t in operands([10, 20, 10], 256, 72, False, 5))
+    x, w = Q.Rows8(xq, xs), Q.Weight8(wq, ws)
+    run = lambda offs: Q.grouped_gemm(x, w, torch.tensor(offs, dtype=torch.int32, device=DEV))
+    whole = run([0, 10, 30, 40])
+    part = run([0, 10, 30, 33])
+    assert same_bits(part[:33], whole[:33]) and (part[33:] == 0).all()
+    late = run([4, 10, 30, 40])
+    assert same_bits(late[4:], whole[4:]) and (late[:4] == 0).all()
+    assert (run([0, 0, 0, 0]) == 0).all()
+    # not what a sort gives, but nothing outside the rows is read or written
+    wild = run([-5, 10, 30, 4000])
+    assert same_bits(wild, whole)
+    falling = run([0, 30, 10, 40])
+    assert torch.isfinite(falling).all()
+    none = Q.grouped_gemm(Q.Rows8(xq[:0], xs[:, :0].contiguous()), w, torch.zeros(4, dtype=torch.int32, device=DEV))
+    assert none.shape == (0, 72)
+
+
+def test_a_row_that_is_not_finite_stays_alone(Q):
+    offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([40, 8], 256, 72, False, 6))
+    x = torch.randn(48, 256, device=DEV)
+    x[3, 200] = float("nan")
+    x[41, 0] = float("inf")
+    got = Q.grouped_gemm(Q.quantize_rows(x), Q.Weight8(wq, ws), offsets)
+    assert got[3].isnan().all() and got[41].isnan().all()
+    assert torch.isfinite(got[[r for r in range(48) if r not in (3, 41)]]).all()
+
+
+def layer(N, E, k, H, I, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(N, H, generator=g).to(dtype).to(DEV)
+    router = (torch.randn(E, H, generator=g) * 0.2).to(dtype).to(DEV)
+    gate_up = (torch.randn(E, 2 * I, H, generator=g) * H ** -0.5).to(dtype).to(DEV)
+    down = (torch.randn(E, H, I, generator=g) * I ** -0.5).to(dtype).to(DEV)
+    return h, router, gate_up, down
+
+
+@pytest.mark.parametrize("N,E,k,H,I,dtype", [(1, 64, 8, 256, 128, BF), (7, 8, 2, 128, 48, HF), (64, 64, 8, 256, 128, HF),
+                                             (333, 64, 8, 256, 144, BF), (2100, 8, 4, 256, 128, BF), (0, 8, 2, 128, 64, BF)])
+def test_the_layer_on_8_bit_experts(Q, N, E, k, H, I, dtype):
+    """moe_layer with Weight8 experts: route, sort, quantise into expert order, product with SwiGLU,
+    quantise, product with router weights, combine: the bits of the operators called one by one,
+    in every mode, with a residual and through GraphedLayer; and near the 16-bit layer."""
+    from switchyard_b200 import kernels, rows
+    h, router, gate_up, down = layer(N, E, k, H, I, dtype)
+    gu8, dn8 = Q.quantize_weight(gate_up, halves=2), Q.quantize_weight(down)
+    out = kernels.moe_layer(h, router, gu8, dn8, k, False)
+    assert out.shape == h.shape and out.dtype == dtype
+    if N == 0:
+        return
+    idx, w, counts, offsets, token, wsorted, pos_of = kernels.route_and_sort(h, router, k, False)
+    plan = rows.SortPlan(counts, offsets, token, pos_of.view(N, k))
+    act = Q.grouped_gemm(Q.quantize_rows(h, plan), gu8, offsets, swiglu=True, dtype=dtype)
+    y = Q.grouped_gemm(Q.quantize_rows(act), dn8, offsets, scale=wsorted, dtype=dtype)
+    assert torch.equal(out, kernels.ext().combine(y, pos_of, idx, N))
+    for mode in ("gemv", "gemm"):
+        assert torch.equal(kernels.moe_layer(h, router, gu8, dn8, k, False, mode), out)
+    assert torch.equal(kernels.experts(h, idx, w, gu8, dn8), out)
+    x = torch.randn_like(h)
+    assert torch.equal(kernels.moe_layer(h, router, gu8, dn8, k, False, residual=x), x + out)
+    graphed = kernels.GraphedLayer(router, gu8, dn8, k, False)
+    for s in (1, 2):
+        hs = layer(N, E, k, H, I, dtype, seed=s)[0]
+        assert torch.equal(graphed(hs), kernels.moe_layer(hs, router, gu8, dn8, k, False))
+    graphed.check()
+    # four operands are rounded to e4m3, each by at most 2^-4 of its values: to first order the result
+    # moves by at most 4 * 2^-4 of what a sum of magnitudes would be; in the 2-norm, by less
+    ref = kernels.moe_layer(h, router, gate_up, down, k, False).double()
+    assert (out.double() - ref).norm() <= 0.25 * ref.norm()
+
+
+def test_streams_and_graphs(Q):
+    """The same call on two streams at once and replayed from a graph, on new inputs."""
+    offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([20, 0, 300], 256, 256, True, 9))
+    w = Q.Weight8(wq, ws)
+    x = torch.randn(320, 256, device=DEV).to(BF)
+    run = lambda: Q.grouped_gemm(Q.quantize_rows(x), w, offsets, swiglu=True)
+    want = run()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for s in streams * 3:
+        with torch.cuda.stream(s):
+            outs.append(run())
+    torch.cuda.synchronize()
+    assert all(same_bits(o, want) for o in outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    x.copy_(torch.randn(320, 256, device=DEV).to(BF))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert same_bits(out, run())
+
+
+def test_refusals(Q):
+    from switchyard_b200 import kernels
+    offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([4, 4], 128, 64, False, 1))
+    x, w = Q.Rows8(xq, xs), Q.Weight8(wq, ws)
+    bad = [dict(x=x._replace(scale=xs.t())), dict(x=x._replace(q=xq.float())), dict(w=w._replace(scale=ws[:1])),
+           dict(w=w._replace(q=wq.cpu())), dict(offsets=offsets[:2]), dict(offsets=offsets.long()), dict(dtype=F32),
+           dict(scale=torch.ones(8, device=DEV)), dict(scale=torch.ones(7, device=DEV, dtype=BF)),
+           dict(swiglu=True, scale=torch.ones(8, device=DEV, dtype=BF))]
+    for change in bad:
+        with pytest.raises(RuntimeError):
+            Q.grouped_gemm(**{**dict(x=x, w=w, offsets=offsets), **change})
+    odd = operands([4, 4], 120, 64, False, 1)
+    with pytest.raises(RuntimeError, match="multiple of 16"):
+        Q.grouped_gemm(Q.Rows8(odd[1].to(DEV), odd[2].to(DEV)), Q.Weight8(odd[3].to(DEV), odd[4].to(DEV)), offsets)
+    for t in (torch.zeros(4, 24, device=DEV), torch.zeros(4, 32), torch.zeros(4, 32, device=DEV).double(), torch.zeros(32, device=DEV)):
+        with pytest.raises(RuntimeError):
+            Q.quantize_rows(t)
+    for t, halves in ((torch.zeros(2, 3, 32, device=DEV), 2), (torch.zeros(3, 32, device=DEV), 1), (torch.zeros(1, 8, 40, device=DEV), 1),
+                      (torch.zeros(1, 9, 32, device=DEV), 3)):
+        with pytest.raises(RuntimeError):
+            Q.quantize_weight(t, halves)
+    with pytest.raises(RuntimeError, match="multiple of 16"):  # experts of width 136: 16-bit only
+        Q.quantize_weight(layer(1, 8, 2, 256, 136, BF)[3])
+    leaf = torch.zeros(4, 32, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        Q.quantize_rows(leaf)
+    with torch.no_grad():
+        Q.quantize_rows(leaf)
+    h, router, gate_up, down = layer(4, 8, 2, 128, 64, BF)
+    gu8 = Q.quantize_weight(gate_up, halves=2)
+    with pytest.raises(RuntimeError, match="both"):
+        kernels.moe_layer(h, router, gu8, down, 2, False)
+    with pytest.raises(RuntimeError, match="mode"):
+        kernels.moe_layer(h, router, gu8, Q.quantize_weight(down), 2, False, "other")
+    with pytest.raises(RuntimeError, match="8-bit"):
+        kernels.ffn(h, None, offsets, None, None, gu8, down, 4, "gemv")

@@ -1,0 +1,115 @@
+"""What the row operators, the quantisers and the 8-bit product refuse before anything touches a
+device (C ABI and Python), and the plain forms the GPU tests compare with."""
+
+import ctypes
+
+import pytest
+import torch
+
+import rows_fp8_cases as rc
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from switchyard_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+P = ctypes.c_void_p(1 << 20)  # an aligned address that a refused call must not look at
+
+
+def refused(lib, rc_, text):
+    assert rc_ == -1 and text in lib.sy_last_error(), (rc_, lib.sy_last_error())
+
+
+def test_row_operators_refuse(lib):
+    refused(lib, lib.sy_permute_rows(P, P, P, 4, 9, 8, 64, 1, P, None), b"top_k")
+    refused(lib, lib.sy_permute_rows(P, P, P, 4, 0, 8, 64, 1, P, None), b"top_k")
+    refused(lib, lib.sy_permute_rows(P, P, P, 4, 2, 8, 60, 1, P, None), b"multiple of 8")
+    refused(lib, lib.sy_permute_rows(P, P, P, 4, 2, 8, 6, 2, P, None), b"multiple of 4")
+    refused(lib, lib.sy_permute_rows(P, P, P, 4, 2, 8, 64, 3, P, None), b"dtype")
+    refused(lib, lib.sy_permute_rows(P, P, P, -1, 2, 8, 64, 1, P, None), b"top_k")
+    refused(lib, lib.sy_permute_rows(P, P, P, 1 << 30, 8, 8, 64, 1, P, None), b"2^31")
+    refused(lib, lib.sy_permute_rows(P, P, P, 4, 2, 0, 64, 1, P, None), b"expert")
+    refused(lib, lib.sy_permute_rows(None, P, P, 4, 2, 8, 64, 1, P, None), b"null")
+    refused(lib, lib.sy_permute_rows(ctypes.c_void_p(8), P, P, 4, 2, 8, 64, 1, P, None), b"aligned")
+    refused(lib, lib.sy_unpermute_rows(P, P, 0, P, 4, 2, 64, 1, P, None), b"weights")
+    refused(lib, lib.sy_unpermute_rows(P, P, 1, P, 4, 2, 64, 2, P, None), b"weights")
+    refused(lib, lib.sy_unpermute_rows(P, None, 0, None, 4, 2, 64, 1, P, None), b"null")
+    refused(lib, lib.sy_unpermute_rows_grad(P, P, P, 0, P, P, 4, 2, 8, 64, 1, P, P, None), b"weights")
+    refused(lib, lib.sy_unpermute_rows_grad(P, None, P, 1, P, P, 4, 2, 8, 64, 1, P, P, None), b"null")
+    # nothing to do: no pointer is needed
+    assert lib.sy_permute_rows(None, None, None, 0, 2, 8, 64, 1, None, None) == 0
+    assert lib.sy_unpermute_rows(None, None, 0, None, 0, 2, 64, 1, None, None) == 0
+    assert lib.sy_unpermute_rows_grad(None, None, None, 0, None, None, 4, 2, 8, 64, 1, None, None, None) == 0
+
+
+def test_quantisers_and_the_product_refuse(lib):
+    refused(lib, lib.sy_quantize_rows(P, None, None, 4, 2, 0, 64, 1, P, P, None), b"one place")
+    refused(lib, lib.sy_quantize_rows(P, P, P, 4, 2, 8, 40, 1, P, P, None), b"multiple of 16")
+    refused(lib, lib.sy_quantize_rows(P, P, P, 4, 9, 8, 64, 1, P, P, None), b"top_k")
+    refused(lib, lib.sy_quantize_rows(P, P, None, 4, 2, 8, 64, 1, P, P, None), b"null")
+    refused(lib, lib.sy_quantize_rows(P, P, P, 4, 2, 8, 64, 7, P, P, None), b"dtype")
+    refused(lib, lib.sy_quantize_weight(P, 1, 0, 64, 1, P, P, None), b"rows")
+    refused(lib, lib.sy_quantize_weight(P, 1 << 20, 8, 64, 1, P, P, None), b"matrices")
+    refused(lib, lib.sy_quantize_weight(P, 1, 8, 40, 1, P, P, None), b"multiple of 16")
+    args = lambda E=8, rows=4, n=64, k=128, sw=0, scale=None, dt=1, tile=0, x=P: (x, P, P, P, P, E, rows, n, k, sw, scale, P, dt,
+                                                                               tile, None)
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(E=257)), b"experts")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(k=120)), b"multiple of 16")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(n=60)), b"multiple of 8")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(sw=1, scale=P)), b"separate")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(dt=2)), b"dtype")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(tile=4)), b"tile")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(x=None)), b"null")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(x=ctypes.c_void_p(8))), b"aligned")
+    assert lib.sy_grouped_gemm_fp8(*args(rows=0, x=None)) == 0
+    refused(lib, lib.sy_sort_by_expert(P, P, 8, 2, 8, 0, P, P, P, None, P, None, 0, None), b"null")
+
+
+def test_tensors_on_the_host_are_refused(lib):
+    """There is no CPU path: every public call says so instead of computing something else."""
+    from switchyard_b200 import fp8, rows
+    idx = torch.zeros(4, 2, dtype=torch.int32)
+    plan = rows.SortPlan(torch.zeros(8, dtype=torch.int32), torch.zeros(9, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), idx)
+    x, w = torch.zeros(4, 64), torch.zeros(4, 2)
+    w8 = fp8.Weight8(torch.zeros(2, 64, 64).to(torch.float8_e4m3fn), torch.zeros(2, 1, 1))
+    x8 = fp8.Rows8(torch.zeros(4, 64).to(torch.float8_e4m3fn), torch.zeros(1, 4))
+    for call in (lambda: rows.plan(idx, 8), lambda: rows.permute_rows(x, plan), lambda: rows.unpermute_rows(torch.zeros(8, 64), w, plan),
+                 lambda: fp8.quantize_rows(x), lambda: fp8.quantize_rows(x, plan), lambda: fp8.quantize_weight(torch.zeros(2, 64, 64)),
+                 lambda: fp8.grouped_gemm(x8, w8, torch.zeros(3, dtype=torch.int32)),
+                 lambda: rows.permute_rows(x.requires_grad_(), plan)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_the_plain_quantiser_is_torchs_e4m3(lib):
+    """nearest8 against torch's own conversion on every 16-bit value it can take, ties included."""
+    v = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(torch.float16).float()
+    v = v[v.abs() <= 448]
+    assert torch.equal(rc.nearest8(v), v.to(torch.float8_e4m3fn).double())
+    q, s = rc.quantize64(torch.zeros(3, 130), 1)
+    assert (q == 0).all() and torch.equal(s, torch.full((3, 2), rc.TINY) / torch.tensor(448.0))
+
+
+def test_the_plain_plan_is_the_sort(lib):
+    from oracle import moe_oracle as mo
+    idx = rc.choices(50, 4, 16, 1)
+    offsets, pos = rc.places(idx, 16)
+    want = mo.sort_by_expert(idx, torch.zeros(50, 4).half(), 16)
+    assert torch.equal(offsets.int(), want[1]) and torch.equal(pos.flatten().int(), want[4])
+
+
+def test_dequantize_is_the_layout(lib):
+    from switchyard_b200 import fp8
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(5, 144, generator=g)
+    q, s = rc.quantize64(x, 1)
+    r8 = fp8.Rows8(q.float().to(torch.float8_e4m3fn), s.t().contiguous())
+    assert ((r8.dequantize() - x).abs() <= x.abs() * (2.0 ** -4 + 2.0 ** -22) + 2.0 ** -10 * 6 / 448).all()
+    w = torch.randn(2, 272, 144, generator=g)
+    parts = [rc.quantize64(p, 128) for p in w.view(4, 136, 144)]
+    w8 = fp8.Weight8(torch.stack([a for a, _ in parts]).view(2, 272, 144).float().to(torch.float8_e4m3fn),
+                     torch.stack([b for _, b in parts]).view(2, 4, 2))
+    assert ((w8.dequantize(halves=2) - w).abs() <= w.abs() * (2.0 ** -4 + 2.0 ** -22) + 2.0 ** -10 * 6 / 448).all()
