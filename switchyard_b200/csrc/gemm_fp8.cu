@@ -14,8 +14,11 @@
 // Warps: 0 TMA producer, 1 MMA issuer, 2-3 spare (they clear rows that belong to no expert), 4-11 promotion and epilogue.
 // Tiles as in gemm.cu: numbered on the device from `offsets`, expert-major, dealt round-robin to
 // a persistent grid. Token rows are the MMA's M operand (128, or 256 over a pair of CTAs), weight
-// rows its N operand; with SwiGLU the N rows are [gate | up | gate | up] quarters of the same
-// output columns, so that a thread finds a gate value and its up value in its own registers.
+// rows its N operand, in two halves of WR / 2: consecutive rows, or with SwiGLU the gate rows and the
+// up rows of the same columns. A thread takes the same quarter of the columns out of either half:
+// it finds a gate value and its up value in its own registers, and each half of the tile is one
+// TMA box (a box takes its thread about 130 clocks to issue, however small: six to eight boxes a
+// stage took twice as long as the multiplication).
 #include <cuda.h>
 
 #include <atomic>
@@ -29,10 +32,12 @@ namespace sy {
 
 constexpr int G8_BLOCK = 128;                    // k per scale and per stage: one 128-byte swizzle atom
 constexpr int G8_XR = 128;                       // token rows a CTA stages
-constexpr int G8_XBOX = 32;                      // token rows per TMA box: only boxes with rows of the tile are loaded
+constexpr int G8_XFEW = 32;                      // token rows of the small TMA box, for tiles of at most two of them
 constexpr int G8_MAX_E = 256;
 constexpr int G8_THREADS = 12 * 32;
 constexpr int G8_PROMOTERS = 8;                  // warps
+constexpr int G8_AHEAD = 6, G8_SLOTS = 8;        // k blocks that a scale is asked for before its use; slots of the ring
+constexpr int G8_SLOT = 32 + 2;                  // a warp's scales of one k block: its rows' and the weights' two
 constexpr int G8_RING_BYTES = 192 * 1024;
 constexpr int G8_SMEM = G8_RING_BYTES + 1024;    // room to align the ring to 1024
 
@@ -41,8 +46,8 @@ template <int WR, bool PAIR> struct Shape8 {
   static constexpr int CTAS = PAIR ? 2 : 1;
   static constexpr int BM = G8_XR * CTAS;                 // token rows per tile
   static constexpr int WRC = WR / CTAS;                   // weight rows a CTA stages
-  static constexpr int WBOX = WR / 4;                     // weight rows per TMA box (a quarter of the tile)
-  static constexpr int W_BOXES = WRC / WBOX;
+  static constexpr int WBOX = WR / 2;                     // weight rows per TMA box: a half of the tile
+  static constexpr int W_BOXES = WRC / WBOX;              // PAIR: each CTA has one of the halves
   static constexpr int X_BYTES = G8_XR * G8_BLOCK;
   static constexpr int STAGE_BYTES = X_BYTES + WRC * G8_BLOCK;
   static constexpr int STAGES = G8_RING_BYTES / STAGE_BYTES;
@@ -57,7 +62,8 @@ static_assert(4 * G8_REGS_FEW + 8 * G8_REGS_MANY <= 12 * G8_REGS_LAUNCH, "regist
 
 struct Gemm8Args {
   CUtensorMap wmap;   // [experts * halves * Nout, K] e4m3, box 128 k x WBOX
-  CUtensorMap xmap;   // [rows, K] e4m3, box 128 k x 32
+  CUtensorMap xmap;   // [rows, K] e4m3, box 128 k x 128
+  CUtensorMap xfew;   // the same, box 128 k x 32
   const float* xscale;  // [k blocks][rows]
   const float* wscale;  // [experts][halves * n blocks][k blocks]
   const int* offsets;   // [experts + 1]
@@ -90,6 +96,9 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
       "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ void cp_async_4(float* dst_smem, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst_smem)), "l"(src) : "memory");
+}
 // 32 lanes x 32 consecutive columns of tensor memory.
 __device__ __forceinline__ void tmem_ld_x32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
@@ -112,20 +121,46 @@ __device__ __forceinline__ void tmem_ld_wait_x32(uint32_t (&r)[32]) {
                :
                : "memory");
 }
-// acc += part * f for two float32 values at once.
-__device__ __forceinline__ void fma2(float2& acc, uint32_t lo, uint32_t hi, uint64_t ff) {
-  asm("{\n\t.reg .b64 p, a;\n\t"
-      "mov.b64 p, {%2, %3};\n\t"
-      "mov.b64 a, {%0, %1};\n\t"
-      "fma.rn.f32x2 a, p, %4, a;\n\t"
-      "mov.b64 {%0, %1}, a;\n\t}"
-      : "+f"(acc.x), "+f"(acc.y)
+// acc += part * f for two float32 values at once. The accumulators are 64-bit values throughout, so
+// that they stay in aligned register pairs.
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t ff) {
+  asm("{\n\t.reg .b64 p;\n\t"
+      "mov.b64 p, {%1, %2};\n\t"
+      "fma.rn.f32x2 %0, p, %3, %0;\n\t}"
+      : "+l"(acc)
       : "r"(lo), "r"(hi), "l"(ff));
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
 }
 __device__ __forceinline__ uint64_t twice(float f) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(f));
   return r;
+}
+
+// Arrives on a barrier of the pair's leader. What it publishes is that tensor-memory reads are done,
+// which tcgen05.wait::ld and the tcgen05 fence before it have settled; so it releases at CTA scope
+// only. A release at cluster scope also waits for the thread's loads in flight (the next blocks'
+// scales), which cost about 600 clocks per k block: 682 -> 425 us for 8192 tokens of the
+// benchmark's layer.
+__device__ __forceinline__ void arrive_leader(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Whether the barrier's phase is over; does not wait.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 struct Tile8 {
@@ -160,6 +195,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
   __shared__ uint32_t s_tmem;
   __shared__ int s_begin[G8_MAX_E], s_end[G8_MAX_E];
   __shared__ int s_tile_start[G8_MAX_E + 2];
+  __shared__ float s_scale[G8_PROMOTERS][G8_SLOTS][G8_SLOT];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* stages =
@@ -187,6 +223,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
     fence_barrier_init();
     prefetch_tensormap(&args.wmap);
     prefetch_tensormap(&args.xmap);
+    prefetch_tensormap(&args.xfew);
   }
   if (warp == 1) {
     if (PAIR) {
@@ -240,20 +277,23 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
       bool alive = true;
       for (int t = unit; t < total_tiles && alive; t += units) {
         const Tile8 tile = locate_tile8<S::BM>(t, cursor, s_tile_start, s_begin, s_end);
-        auto boxes_of = [&](int c) { return (min(max(tile.nvalid - c * G8_XR, 0), G8_XR) + G8_XBOX - 1) / G8_XBOX; };
-        const int x_boxes = boxes_of(cr);
-        const uint32_t bytes =
-            WR * G8_BLOCK + (x_boxes + (PAIR ? boxes_of(cr ^ 1) : 0)) * (G8_XBOX * G8_BLOCK);  // of all CTAs of the tile
+        // token rows: one box of 128, or one or two of 32 where the tile has no more
+        auto rows_of = [&](int c) { return min(max(tile.nvalid - c * G8_XR, 0), G8_XR); };
+        auto x_bytes = [&](int n) {
+          return n > 2 * G8_XFEW ? S::X_BYTES : (n + G8_XFEW - 1) / G8_XFEW * (G8_XFEW * G8_BLOCK);
+        };
+        const int mine = rows_of(cr);
+        const bool few = mine <= 2 * G8_XFEW;
+        const int x_boxes = few ? (mine + G8_XFEW - 1) / G8_XFEW : 1;
+        const uint32_t bytes = WR * G8_BLOCK + x_bytes(mine) + (PAIR ? x_bytes(rows_of(cr ^ 1)) : 0);  // of all CTAs of the tile
         const bool is_w = lane < S::W_BOXES, is_x = !is_w && lane - S::W_BOXES < x_boxes;
-        const int b = is_w ? cr * S::W_BOXES + lane : lane - S::W_BOXES;  // quarter of the weight rows, or box of token rows
-        int y;
-        if (is_w) {
-          const int colbase = tile.cb * tile_cols;
-          y = swiglu ? (tile.e * 2 + (b & 1)) * Nout + colbase + (b >> 1) * S::WBOX : tile.e * Nout + colbase + b * S::WBOX;
-        } else {
-          y = tile.row0 + cr * G8_XR + b * G8_XBOX;
-        }
-        const int off = is_w ? S::X_BYTES + lane * (S::WBOX * G8_BLOCK) : b * (G8_XBOX * G8_BLOCK);
+        const int b = is_w ? cr + lane : lane - S::W_BOXES;  // half of the weight rows, or box of token rows
+        const int colbase = tile.cb * tile_cols;
+        const int y = is_w ? (swiglu ? (tile.e * 2 + b) * Nout + colbase : tile.e * Nout + colbase + b * S::WBOX)
+                           : tile.row0 + cr * G8_XR + b * G8_XFEW;
+        const int off = is_w ? S::X_BYTES + lane * (S::WBOX * G8_BLOCK) : b * (G8_XFEW * G8_BLOCK);
+        const void* map = is_w ? static_cast<const void*>(&args.wmap)
+                               : few ? static_cast<const void*>(&args.xfew) : static_cast<const void*>(&args.xmap);
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % STAGES, use = it / STAGES;
           int ok = 1;
@@ -268,7 +308,6 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
             break;
           }
           if (is_w || is_x) {
-            const void* map = is_w ? static_cast<const void*>(&args.wmap) : static_cast<const void*>(&args.xmap);
             unsigned char* dst = stages + (size_t)s * S::STAGE_BYTES + off;
             if (PAIR) tma_load_2d_pair(dst, map, kb * G8_BLOCK, y, cluster_map(&full_bar[s], 0));
             else tma_load_2d(dst, map, kb * G8_BLOCK, y, &full_bar[s]);
@@ -279,46 +318,49 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
         for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full_bar[j % STAGES], (j / STAGES) & 1, 10000000ull);
     } else if (warp == 1) {
       // -------------------------------------------------------------- MMA issuer (PAIR: the leader's, for both CTAs)
-      if (lane == 0 && cr == 0) {
+      // The whole warp walks the k blocks (so that descriptors and loop counters stay in uniform
+      // registers), one elected lane issues; the next block's two barriers are looked at while this
+      // block's MMAs are on their way.
+      if (cr == 0) {
         const uint32_t ring_lo = umma_desc_lo(smem_u32(stages));
         const uint32_t idesc = umma_idesc(0, S::BM, WR);  // format 0 is e4m3 in this kind
-        int it = 0, cursor = 0;
-        bool alive = true;
-        for (int t = unit; t < total_tiles && alive; t += units) {
-          locate_tile8<S::BM>(t, cursor, s_tile_start, s_begin, s_end);
-          for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-            const int s = it % STAGES, buf = it & 1, use = it >> 1;
-            bool ok = true;
-            if (use > 0) ok = PAIR ? mbar_wait_cluster(&part_empty[buf], (use - 1) & 1, wait_ns)
-                                   : mbar_wait(&part_empty[buf], (use - 1) & 1, wait_ns);
-            if (!ok) {
-              *status = DS_TIMEOUT_TMEM;
-              alive = false;
-              break;
-            }
-            ok = PAIR ? mbar_wait_cluster(&full_bar[s], (it / STAGES) & 1, wait_ns)
-                      : mbar_wait(&full_bar[s], (it / STAGES) & 1, wait_ns);
-            if (!ok) {
-              *status = DS_TIMEOUT_FULL;
-              alive = false;
-              break;
-            }
-            tc_fence_after_sync();
-            const uint32_t x_lo = ring_lo + s * (S::STAGE_BYTES >> 4), w_lo = x_lo + (S::X_BYTES >> 4);
-            const uint32_t d = tmem + buf * WR;
+        const int n = total_tiles > unit ? ((total_tiles - unit + units - 1) / units) * k_blocks : 0;
+        int s = 0;
+        uint32_t phase = 0;
+        bool drained = true, filled = false;
+        for (int it = 0; it < n; ++it) {
+          const int buf = it & 1;
+          if (!drained && !mbar_wait(&part_empty[buf], ((it >> 1) - 1) & 1, wait_ns)) {
+            *status = DS_TIMEOUT_TMEM;
+            break;
+          }
+          if (!filled && !mbar_wait(&full_bar[s], phase, wait_ns)) {
+            *status = DS_TIMEOUT_FULL;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t x_lo = ring_lo + s * (S::STAGE_BYTES >> 4), w_lo = x_lo + (S::X_BYTES >> 4);
+          const uint32_t d = tmem + buf * WR;
+          const int s_next = s + 1 == STAGES ? 0 : s + 1;
+          const uint32_t phase_next = s_next ? phase : phase ^ 1;
+          if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {  // 32 k = 32 bytes inside the 128-byte rows
               if (PAIR) umma_f8_pair(d, x_lo + ks * 2, w_lo + ks * 2, UMMA_DESC_HI_K_SW128, idesc, ks != 0);
               else umma_f8(d, x_lo + ks * 2, w_lo + ks * 2, UMMA_DESC_HI_K_SW128, idesc, ks != 0);
             }
             if (PAIR) {
-              umma_commit_pair(&empty_bar[s], 3);
               umma_commit_pair(&part_full[buf], 3);
+              umma_commit_pair(&empty_bar[s], 3);
             } else {
-              umma_commit(&empty_bar[s]);
               umma_commit(&part_full[buf]);
+              umma_commit(&empty_bar[s]);
             }
           }
+          __syncwarp();
+          drained = it < 1 || mbar_test(&part_empty[buf ^ 1], (((it + 1) >> 1) - 1) & 1);
+          filled = mbar_test(&full_bar[s_next], phase_next);
+          s = s_next, phase = phase_next;
         }
       }
     } else {
@@ -336,60 +378,106 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
     const int q = warp & 3, g = (warp - 4) >> 2;  // quarter of the lanes; half of the tile's columns
     const int trow = cr * G8_XR + q * 32 + lane;
     const int n_blocks = (Nout + G8_BLOCK - 1) / G8_BLOCK;
-    const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + g * ACC;
+    const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + g * (ACC / 2);
+    // accumulator columns 32 c, ... of the thread: a quarter of the tile's first half, then of its second
+    auto column_of = [](int c) { return c < ACC / 64 ? c * 32 : WR / 2 + (c - ACC / 64) * 32; };
+    // first output column of the thread's quarter of the tile's first half
+    auto col_of = [&](const Tile8& tile) { return tile.cb * tile_cols + g * (ACC / 2); };
+    // Scales: every thread copies its row's, two lanes the weights' two, into slots of the warp's own,
+    // G8_AHEAD k blocks before they are used (across tiles), asynchronously and without registers.
+    float (*slots)[G8_SLOT] = s_scale[warp - 4];
+    Tile8 ptile;
+    int pt = unit, pkb = 0, pcursor = 0, ahead = 0;
+    const float *px = nullptr, *pw = nullptr;
+    auto enter = [&]() {  // the scales of tile pt
+      ptile = locate_tile8<S::BM>(pt, pcursor, s_tile_start, s_begin, s_end);
+      px = args.xscale + ptile.row0 + (trow < ptile.nvalid ? trow : 0);
+      const int col = col_of(ptile);
+      const int nb = swiglu ? (lane & 1) * n_blocks + min(col / G8_BLOCK, n_blocks - 1)
+                            : min((col + (lane & 1) * (WR / 2)) / G8_BLOCK, n_blocks - 1);
+      pw = args.wscale + ((size_t)ptile.e * (swiglu ? 2 : 1) * n_blocks + nb) * k_blocks;
+    };
+    auto prefetch = [&]() {
+      if (pt < total_tiles) {
+        float* slot = slots[ahead & (G8_SLOTS - 1)];
+        cp_async_4(slot + lane, px);
+        if (lane < 2) cp_async_4(slot + 32 + lane, pw);
+        px += args.rows, ++pw;
+        if (++pkb == k_blocks) {
+          pkb = 0, pt += units;
+          if (pt < total_tiles) enter();
+        }
+      }
+      ++ahead;
+      cp_async_commit();
+    };
+    if (pt < total_tiles) enter();
+    for (int i = 0; i < G8_AHEAD; ++i) prefetch();
     int it = 0, cursor = 0;
     bool alive = true;
     for (int t = unit; t < total_tiles; t += units) {
       const Tile8 tile = locate_tile8<S::BM>(t, cursor, s_tile_start, s_begin, s_end);
       const bool busy = cr * G8_XR + q * 32 < tile.nvalid;  // the warp has rows of this tile
       const bool valid = trow < tile.nvalid;
-      const int row = tile.row0 + (valid ? trow : 0);
-      // output columns [col, col + ACC), with SwiGLU [col, col + ACC / 2)
-      const int col = tile.cb * tile_cols + g * (swiglu ? ACC / 2 : ACC);
-      const int nb = min(col / G8_BLOCK, n_blocks - 1);
-      const float* sx = args.xscale + row;
-      const float* sw0 = args.wscale + ((size_t)tile.e * (swiglu ? 2 : 1) * n_blocks + nb) * k_blocks;
-      const float* sw1 = sw0 + (swiglu ? (size_t)n_blocks * k_blocks : 0);
-      float2 acc[ACC / 2];
+      const int row = tile.row0 + trow, col = col_of(tile);
+      uint64_t acc[ACC / 2];
 #pragma unroll
-      for (int i = 0; i < ACC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-      // the scales of the next two blocks are on their way while this one is promoted
-      float x0 = __ldg(sx), a0 = __ldg(sw0), b0 = __ldg(sw1), x1 = 0.f, a1 = 0.f, b1 = 0.f;
-      if (k_blocks > 1) x1 = __ldg(sx + args.rows), a1 = __ldg(sw0 + 1), b1 = __ldg(sw1 + 1);
-      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-        const int buf = it & 1, use = it >> 1;
-        const uint64_t f0 = twice(x0 * a0), f1 = twice(x0 * b0);
-        x0 = x1, a0 = a1, b0 = b1;
-        if (kb + 2 < k_blocks) {
-          x1 = __ldg(sx + (size_t)(kb + 2) * args.rows);
-          a1 = __ldg(sw0 + kb + 2);
-          b1 = __ldg(sw1 + kb + 2);
-        }
-        if (alive && !mbar_wait(&part_full[buf], use & 1, wait_ns)) {
+      for (int i = 0; i < ACC / 2; ++i) acc[i] = 0;
+      // Waits for the partial product of k block `it`. A warp that gave up goes on without waiting.
+      auto open = [&]() {
+        if (alive && !mbar_wait(&part_full[it & 1], (it >> 1) & 1, wait_ns)) {
           *status = DS_TIMEOUT_MMA;
           alive = false;
         }
-        alive = __all_sync(0xffffffffu, alive);
-        if (!alive) continue;
+        __syncwarp();
         tc_fence_after_sync();
-        if (busy) {
-          const uint32_t from = taddr + buf * WR;
-          uint32_t v[2][32];
-          tmem_ld_x32(from, v[0]);
-#pragma unroll
-          for (int c = 0; c < ACC / 32; ++c) {
-            tmem_ld_wait_x32(v[c & 1]);
-            if (c + 1 < ACC / 32) tmem_ld_x32(from + (c + 1) * 32, v[(c + 1) & 1]);
-            const uint64_t f = c < ACC / 64 ? f0 : f1;  // with SwiGLU the first half are gate columns, the second up
-#pragma unroll
-            for (int j = 0; j < 16; ++j) fma2(acc[c * 16 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], f);
-          }
-        }
+      };
+      // All of it is in registers: the buffer may be overwritten.
+      auto close = [&]() {
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          if (PAIR) mbar_arrive_cluster(cluster_map(&part_empty[buf], 0));
-          else mbar_arrive(&part_empty[buf]);
+          if (PAIR) arrive_leader(cluster_map(&part_empty[it & 1], 0));
+          else mbar_arrive(&part_empty[it & 1]);
+        }
+      };
+      if (!busy) {
+        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+          prefetch();
+          open();
+          close();
+        }
+        continue;
+      }
+      uint32_t v[2][32];
+      open();
+      tmem_ld_x32(taddr + (it & 1) * WR + column_of(0), v[0]);
+#pragma unroll 1
+      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+        prefetch();
+        cp_async_wait<G8_AHEAD>();
+        __syncwarp();
+        const float* slot = slots[it & (G8_SLOTS - 1)];
+        const float x = slot[lane];
+        const uint64_t f0 = twice(x * slot[32]), f1 = twice(x * slot[33]);
+        const uint32_t from = taddr + (it & 1) * WR;
+#pragma unroll
+        for (int c = 0; c < ACC / 32; ++c) {
+          tmem_ld_wait_x32(v[c & 1]);
+          if (c + 1 < ACC / 32) {
+            tmem_ld_x32(from + column_of(c + 1), v[(c + 1) & 1]);
+          } else {  // the next block's first columns are on their way during the last multiply-adds
+            close();
+            if (kb + 1 < k_blocks) {
+              ++it;
+              open();
+              tmem_ld_x32(taddr + (it & 1) * WR + column_of(0), v[0]);
+              --it;
+            }
+          }
+          const uint64_t f = c < ACC / 64 ? f0 : f1;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) fma2(acc[c * 16 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], f);
         }
       }
       if (!alive || !valid) continue;
@@ -397,7 +485,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
       const float s = args.scale ? Elem<T>::to_f(static_cast<const T*>(args.scale)[row]) : 1.f;
       const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
       constexpr int VALUES = 16;
-      auto store16 = [&](int c, const float (&f)[VALUES]) {
+      auto store16 = [&](int c, const float (&f)[VALUES]) {  // columns col + c, ...
         uint32_t o[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -417,7 +505,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
           float f[VALUES];
 #pragma unroll
           for (int j = 0; j < VALUES / 2; ++j) {
-            const float2 gate = acc[c / 2 + j], up = acc[ACC / 4 + c / 2 + j];
+            const float2 gate = both(acc[c / 2 + j]), up = both(acc[ACC / 4 + c / 2 + j]);
             f[2 * j] = swiglu32(gate.x, up.x);
             f[2 * j + 1] = swiglu32(gate.y, up.y);
           }
@@ -429,10 +517,11 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
           float f[VALUES];
 #pragma unroll
           for (int j = 0; j < VALUES / 2; ++j) {
-            f[2 * j] = acc[c / 2 + j].x * s;
-            f[2 * j + 1] = acc[c / 2 + j].y * s;
+            const float2 a = both(acc[c / 2 + j]);
+            f[2 * j] = a.x * s;
+            f[2 * j + 1] = a.y * s;
           }
-          store16(c, f);
+          store16(c < ACC / 2 ? c : WR / 2 + c - ACC / 2, f);
         }
       }
     }
@@ -502,7 +591,9 @@ static int launch8(Gemm8Args a, const void* x, const void* w, cudaStream_t strea
   const uint64_t w_rows = (uint64_t)a.experts * (a.swiglu ? 2 : 1) * a.Nout;
   rc = tensor_map_2d(&a.wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, w_rows, (uint64_t)a.K, S::WBOX, G8_BLOCK);
   if (rc != SY_OK) return rc;
-  rc = tensor_map_2d(&a.xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XBOX, G8_BLOCK);
+  rc = tensor_map_2d(&a.xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XR, G8_BLOCK);
+  if (rc != SY_OK) return rc;
+  rc = tensor_map_2d(&a.xfew, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XFEW, G8_BLOCK);
   if (rc != SY_OK) return rc;
   auto kern = gemm8_kernel<T, WR, PAIR>;
   if (PAIR) return launch_cluster_kernel(kern, 2, 2 * units, G8_THREADS, G8_SMEM, stream, "grouped_gemm_fp8 launch", a);
