@@ -11,7 +11,7 @@
 // columns. Both factors of a step are the same for all of a thread's columns of one weight block,
 // so the promotion costs one packed multiply-add per two values.
 //
-// Warps: 0 TMA producer, 1 MMA issuer, 2-3 spare (they clear rows that belong to no expert), 4-11 promotion and epilogue.
+// Warps: 0 TMA producer, 1-2 MMA issuers, 3 scales, 4-11 promotion and epilogue.
 // Tiles as in gemm.cu: numbered on the device from `offsets`, expert-major, dealt round-robin to
 // a persistent grid. Token rows are the MMA's M operand (128, or 256 over a pair of CTAs), weight
 // rows its N operand, in two halves of WR / 2: consecutive rows, or with SwiGLU the gate rows and the
@@ -34,10 +34,8 @@ constexpr int G8_BLOCK = 128;                    // k per scale and per stage: o
 constexpr int G8_XR = 128;                       // token rows a CTA stages
 constexpr int G8_XFEW = 32;                      // token rows of the small TMA box, for tiles of at most two of them
 constexpr int G8_MAX_E = 256;
-constexpr int G8_THREADS = 12 * 32;
-constexpr int G8_PROMOTERS = 8;                  // warps
-constexpr int G8_AHEAD = 6, G8_SLOTS = 8;        // k blocks that a scale is asked for before its use; slots of the ring
-constexpr int G8_SLOT = 32 + 2;                  // a warp's scales of one k block: its rows' and the weights' two
+constexpr int G8_SLOTS = 4;                      // k blocks whose scales are in shared memory
+constexpr int G8_HELPERS = 4;                    // warps before the promoters: TMA, two for MMA, scales
 constexpr int G8_RING_BYTES = 192 * 1024;
 constexpr int G8_SMEM = G8_RING_BYTES + 1024;    // room to align the ring to 1024
 
@@ -52,13 +50,14 @@ template <int WR, bool PAIR> struct Shape8 {
   static constexpr int STAGE_BYTES = X_BYTES + WRC * G8_BLOCK;
   static constexpr int STAGES = G8_RING_BYTES / STAGE_BYTES;
   static constexpr int TMEM_COLS = 2 * WR;                // two partial products
-  static constexpr int ACC = WR / 2;                      // columns per promoter thread
-  // 128 accumulators need more registers than 65536 / 384: the four other warps hand theirs over
-  static constexpr bool SPLIT_REGS = ACC > 64;
+  static constexpr int PROMOTERS = 8;                     // warps
+  static constexpr int THREADS = (G8_HELPERS + PROMOTERS) * 32;
+  static constexpr int COLS = WR / 4;                     // columns a promoter thread has of either half
+  // 128 accumulators: the helpers hand some of their registers to the promoters
+  static constexpr bool SPLIT_REGS = COLS > 32;
 };
-constexpr int G8_REGS_FEW = 72, G8_REGS_MANY = 216;       // 4 warps x 72 + 8 warps x 216 <= 12 warps x 168
-constexpr int G8_REGS_LAUNCH = 168;
-static_assert(4 * G8_REGS_FEW + 8 * G8_REGS_MANY <= 12 * G8_REGS_LAUNCH, "register split");
+constexpr int G8_REGS_LAUNCH = 168, G8_REGS_FEW = 88, G8_REGS_MANY = 208;
+static_assert(G8_HELPERS * G8_REGS_FEW + 8 * G8_REGS_MANY <= (G8_HELPERS + 8) * G8_REGS_LAUNCH, "register split");
 
 struct Gemm8Args {
   CUtensorMap wmap;   // [experts * halves * Nout, K] e4m3, box 128 k x WBOX
@@ -69,7 +68,7 @@ struct Gemm8Args {
   const int* offsets;   // [experts + 1]
   const void* scale;    // [rows] or null
   void* C;              // [rows, Nout]
-  int experts, rows, Nout, K, swiglu;
+  int experts, rows, Nout, K;
   int* status;
   unsigned long long wait_ns;
 };
@@ -96,30 +95,16 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
       "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void cp_async_4(float* dst_smem, const float* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst_smem)), "l"(src) : "memory");
-}
-// 32 lanes x 32 consecutive columns of tensor memory.
-__device__ __forceinline__ void tmem_ld_x32(uint32_t addr, uint32_t (&r)[32]) {
+// 32 lanes x 16 consecutive columns of tensor memory, and the wait for them in the same statement: the
+// registers are not to be touched before it.
+__device__ __forceinline__ void tmem_get_x16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr)
       : "memory");
-}
-// Waits for this thread's tensor-memory loads. Naming the registers keeps their uses behind the wait.
-__device__ __forceinline__ void tmem_ld_wait_x32(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
 }
 // acc += part * f for two float32 values at once. The accumulators are 64-bit values throughout, so
 // that they stay in aligned register pairs.
@@ -129,6 +114,26 @@ __device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, ui
       "fma.rn.f32x2 %0, p, %3, %0;\n\t}"
       : "+l"(acc)
       : "r"(lo), "r"(hi), "l"(ff));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two float32 values rounded to T, the first in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return reinterpret_cast<const uint32_t&>(v);
 }
 __device__ __forceinline__ float2 both(uint64_t v) {
   float2 f;
@@ -150,43 +155,46 @@ __device__ __forceinline__ void arrive_leader(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// Whether the barrier's phase is over; does not wait.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 struct Tile8 {
   int e, cb, row0, nvalid;
 };
 
+// Tile t of the launch, found by a whole warp. `cursor` walks the experts; start[E] is the tiles' number.
 template <int BM>
-__device__ __forceinline__ Tile8 locate_tile8(int t, int& cursor, const int* start, const int* begin, const int* end) {
-  while (start[cursor + 1] <= t) ++cursor;
+__device__ __forceinline__ Tile8 locate_tile8(int t, int& cursor, int E, const int* start, const int* begin, const int* end) {
+  const int lane = threadIdx.x & 31;
+  for (;;) {  // experts that end at or before t, 32 at a time
+    const int e = cursor + 1 + lane;
+    const unsigned past = __ballot_sync(0xffffffffu, e <= E && start[e] <= t);
+    cursor += __popc(past);
+    if (past != 0xffffffffu) break;
+  }
   const int local = t - start[cursor], n = end[cursor] - begin[cursor], row_tiles = (n + BM - 1) / BM;
+  // local / row_tiles: below 2^20 the float quotient of local + 1/2 cannot reach the next integer
+  const int cb = local < (1 << 20) ? (int)(((float)local + 0.5f) * rcp_approx((float)row_tiles)) : local / row_tiles;
   Tile8 tile;
   tile.e = cursor;
-  tile.cb = local / row_tiles;
-  tile.row0 = begin[cursor] + (local % row_tiles) * BM;
+  tile.cb = cb;
+  tile.row0 = begin[cursor] + (local - cb * row_tiles) * BM;
   tile.nvalid = min(BM, end[cursor] - tile.row0);
   return tile;
 }
 
-// silu(g) * u. exp and the division are the approximate ones: within about 2^-21, far inside the
-// 16-bit rounding that follows.
-__device__ __forceinline__ float swiglu32(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// silu(g) * u for two columns: the reciprocals of both 1 + exp(-g) come from the one of their
+// product (the special-function unit is what an epilogue waits for). exp and the reciprocal are the
+// approximate ones, within about 2^-21: far inside the 16-bit rounding that follows. exp(-g) is
+// kept below 2^62 so that the product stays finite: below g = -43 sigmoid is taken as 2^-62.
+__device__ __forceinline__ float2 swiglu32(float2 g, float2 u) {
+  constexpr float LOG2E = 1.4426950408889634f;
+  const float d0 = 1.f + exp2_approx(fminf(g.x * -LOG2E, 62.f)), d1 = 1.f + exp2_approx(fminf(g.y * -LOG2E, 62.f));
+  const float r = rcp_approx(d0 * d1);
+  return make_float2(g.x * u.x * (r * d1), g.y * u.y * (r * d0));
+}
 
-template <typename T, int WR, bool PAIR>
-__global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_constant__ Gemm8Args args) {
+template <typename T, int WR, bool PAIR, bool SWIGLU>
+__global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(const __grid_constant__ Gemm8Args args) {
   using S = Shape8<WR, PAIR>;
-  constexpr int STAGES = S::STAGES, ACC = S::ACC;
+  constexpr int STAGES = S::STAGES;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES];
   __shared__ __align__(8) uint64_t empty_bar[STAGES];
@@ -194,19 +202,19 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
   __shared__ __align__(8) uint64_t part_empty[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_begin[G8_MAX_E], s_end[G8_MAX_E];
-  __shared__ int s_tile_start[G8_MAX_E + 2];
-  __shared__ float s_scale[G8_PROMOTERS][G8_SLOTS][G8_SLOT];
+  __shared__ int s_tile_start[G8_MAX_E + 1];
+  __shared__ float2 s_scale[G8_SLOTS][G8_XR];  // per row: its scale times the weights', of either half
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (uniform to the compiler, so that the roles are too)
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   unsigned char* stages =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   int* status = args.status;
   const uint64_t wait_ns = args.wait_ns;
   const int E = args.experts, Nout = args.Nout;
-  const bool swiglu = args.swiglu != 0;
   const int cr = PAIR ? (int)cluster_ctarank() : 0;
   const int unit = PAIR ? (int)blockIdx.x >> 1 : (int)blockIdx.x, units = PAIR ? (int)gridDim.x >> 1 : (int)gridDim.x;
-  const int tile_cols = swiglu ? WR / 2 : WR;
+  const int tile_cols = SWIGLU ? WR / 2 : WR;
   const int col_blocks = (Nout + tile_cols - 1) / tile_cols;
   const int k_blocks = (args.K + G8_BLOCK - 1) / G8_BLOCK;
 
@@ -217,8 +225,8 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
       mbar_init(&empty_bar[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&part_full[b], 1);
-      mbar_init(&part_empty[b], S::CTAS * G8_PROMOTERS);  // PAIR: the leader's, for both CTAs
+      mbar_init(&part_full[b], 2);                           // the MMAs, and this CTA's scales
+      mbar_init(&part_empty[b], S::CTAS * S::PROMOTERS);  // PAIR: the leader's, for both CTAs
     }
     fence_barrier_init();
     prefetch_tensormap(&args.wmap);
@@ -235,7 +243,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
     }
   }
   pdl_wait();
-  for (int e = threadIdx.x; e < E; e += G8_THREADS) {
+  for (int e = threadIdx.x; e < E; e += S::THREADS) {
     // kept inside [0, rows] and ascending whatever the caller's offsets say
     const int b = min(max(args.offsets[e], 0), args.rows), n = min(args.offsets[e + 1], args.rows);
     s_begin[e] = b;
@@ -256,10 +264,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
       if (e < E) s_tile_start[e] = carry + inc - tiles;
       carry += __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (lane == 0) {
-      s_tile_start[E] = carry;
-      s_tile_start[E + 1] = 0x7fffffff;
-    }
+    if (lane == 0) s_tile_start[E] = carry;
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -276,7 +281,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
       int it = 0, cursor = 0;
       bool alive = true;
       for (int t = unit; t < total_tiles && alive; t += units) {
-        const Tile8 tile = locate_tile8<S::BM>(t, cursor, s_tile_start, s_begin, s_end);
+        const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
         // token rows: one box of 128, or one or two of 32 where the tile has no more
         auto rows_of = [&](int c) { return min(max(tile.nvalid - c * G8_XR, 0), G8_XR); };
         auto x_bytes = [&](int n) {
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
         const bool is_w = lane < S::W_BOXES, is_x = !is_w && lane - S::W_BOXES < x_boxes;
         const int b = is_w ? cr + lane : lane - S::W_BOXES;  // half of the weight rows, or box of token rows
         const int colbase = tile.cb * tile_cols;
-        const int y = is_w ? (swiglu ? (tile.e * 2 + b) * Nout + colbase : tile.e * Nout + colbase + b * S::WBOX)
+        const int y = is_w ? (SWIGLU ? (tile.e * 2 + b) * Nout + colbase : tile.e * Nout + colbase + b * S::WBOX)
                            : tile.row0 + cr * G8_XR + b * G8_XFEW;
         const int off = is_w ? S::X_BYTES + lane * (S::WBOX * G8_BLOCK) : b * (G8_XFEW * G8_BLOCK);
         const void* map = is_w ? static_cast<const void*>(&args.wmap)
@@ -316,33 +321,31 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
       }
       if (!alive && cr == 0 && lane == 0)  // the copies already issued land before the block can exit
         for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full_bar[j % STAGES], (j / STAGES) & 1, 10000000ull);
-    } else if (warp == 1) {
-      // -------------------------------------------------------------- MMA issuer (PAIR: the leader's, for both CTAs)
-      // The whole warp walks the k blocks (so that descriptors and loop counters stay in uniform
-      // registers), one elected lane issues; the next block's two barriers are looked at while this
-      // block's MMAs are on their way.
+    } else if (warp <= 2) {
+      // -------------------------------------------------------------- MMA issuers (PAIR: the leader's, for both CTAs)
+      // One warp for either partial product: the k blocks in turn. A wait costs its warp 100 to 250
+      // clocks even when there is nothing to wait for; with one warp for all blocks those came
+      // one after another, 750 clocks a block.
+      // The whole warp walks the blocks (so that descriptors and loop counters stay in uniform
+      // registers), one elected lane issues.
       if (cr == 0) {
         const uint32_t ring_lo = umma_desc_lo(smem_u32(stages));
         const uint32_t idesc = umma_idesc(0, S::BM, WR);  // format 0 is e4m3 in this kind
         const int n = total_tiles > unit ? ((total_tiles - unit + units - 1) / units) * k_blocks : 0;
-        int s = 0;
-        uint32_t phase = 0;
-        bool drained = true, filled = false;
-        for (int it = 0; it < n; ++it) {
-          const int buf = it & 1;
-          if (!drained && !mbar_wait(&part_empty[buf], ((it >> 1) - 1) & 1, wait_ns)) {
-            *status = DS_TIMEOUT_TMEM;
+        const int buf = warp - 1;
+        const uint32_t d = tmem + buf * WR;
+        for (int it = buf; it < n; it += 2) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, wait_ns)) {
+            *status = DS_TIMEOUT_FULL;
             break;
           }
-          if (!filled && !mbar_wait(&full_bar[s], phase, wait_ns)) {
-            *status = DS_TIMEOUT_FULL;
+          if (it >= 2 && !mbar_wait(&part_empty[buf], ((it >> 1) - 1) & 1, wait_ns)) {
+            *status = DS_TIMEOUT_TMEM;
             break;
           }
           tc_fence_after_sync();
           const uint32_t x_lo = ring_lo + s * (S::STAGE_BYTES >> 4), w_lo = x_lo + (S::X_BYTES >> 4);
-          const uint32_t d = tmem + buf * WR;
-          const int s_next = s + 1 == STAGES ? 0 : s + 1;
-          const uint32_t phase_next = s_next ? phase : phase ^ 1;
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {  // 32 k = 32 bytes inside the 128-byte rows
@@ -358,128 +361,123 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
             }
           }
           __syncwarp();
-          drained = it < 1 || mbar_test(&part_empty[buf ^ 1], (((it + 1) >> 1) - 1) & 1);
-          filled = mbar_test(&full_bar[s_next], phase_next);
-          s = s_next, phase = phase_next;
         }
       }
     } else {
-      // -------------------------------------------------------------- rows of no expert are zero
-      const int lo = E ? s_begin[0] : 0, hi = E ? s_end[E - 1] : 0;
-      const int vecs = Nout / 8, who = ((int)blockIdx.x * 2 + (warp - 2)), step = (int)gridDim.x * 2;
-      for (int r = who; r < lo + (args.rows - hi); r += step) {
+      // -------------------------------------------------------------- scales (and the rows of no expert)
+      for (int r = (int)blockIdx.x, lo = s_begin[0], hi = s_end[E - 1]; r < lo + (args.rows - hi); r += (int)gridDim.x) {
         uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(args.C) + (size_t)(r < lo ? r : hi + (r - lo)) * Nout);
-        for (int c = lane; c < vecs; c += 32) row[c] = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = lane; c < Nout / 8; c += 32) row[c] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      // A lane has four of the CTA's rows.
+      const int n_blocks = (Nout + G8_BLOCK - 1) / G8_BLOCK;
+      int t = unit, kb = 0, cursor = 0;
+      const float *px = nullptr, *pw = nullptr;
+      int own[4];
+      auto enter = [&]() {  // the tile of the next block
+        const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = cr * G8_XR + lane + 32 * i;
+          own[i] = r < tile.nvalid ? r : 0;
+        }
+        px = args.xscale + tile.row0;
+        const int col = tile.cb * tile_cols;
+        const int nb = SWIGLU ? (lane & 1) * n_blocks + col / G8_BLOCK
+                              : min((col + (lane & 1) * (WR / 2)) / G8_BLOCK, n_blocks - 1);
+        pw = args.wscale + ((size_t)tile.e * (SWIGLU ? 2 : 1) * n_blocks + nb) * k_blocks;  // lane parity: the half
+      };
+      float x[2][4], w[2];  // asked for two rounds before they are used
+      auto fetch = [&](int i) {
+        if (t >= total_tiles) return;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[i][r] = __ldg(px + own[r]);
+        w[i] = __ldg(pw);
+        px += args.rows, ++pw;
+        if (++kb == k_blocks) {
+          kb = 0, t += units;
+          if (t < total_tiles) enter();
+        }
+      };
+      const int n = total_tiles > unit ? ((total_tiles - unit + units - 1) / units) * k_blocks : 0;
+      if (n) enter();
+      fetch(0);
+      fetch(1);
+      bool alive = true;
+      auto round = [&](int it, int i) {
+        // Block it - 2 has been multiplied, so its predecessor in the same slot has been promoted; and
+        // this block's word cannot be taken for that one's.
+        if (it >= 2 && !mbar_wait(&part_full[i], ((it >> 1) - 1) & 1, wait_ns)) {
+          *status = DS_TIMEOUT_MMA;
+          alive = false;
+          return;
+        }
+        float2* slot = s_scale[it & (G8_SLOTS - 1)];
+        const float w0 = __shfl_sync(0xffffffffu, w[i], 0), w1 = __shfl_sync(0xffffffffu, w[i], 1);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) slot[lane + 32 * r] = make_float2(x[i][r] * w0, x[i][r] * w1);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&part_full[i]);
+        fetch(i);
+      };
+      for (int it = 0; it < n && alive; it += 2) {
+        round(it, 0);
+        if (it + 1 < n && alive) round(it + 1, 1);
       }
     }
   } else {
     // ---------------------------------------------------------------- promotion and epilogue
     if (S::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G8_REGS_MANY));
-    const int q = warp & 3, g = (warp - 4) >> 2;  // quarter of the lanes; half of the tile's columns
+    const int q = warp & 3, g = (warp - G8_HELPERS) >> 2;  // quarter of the lanes; quarter of the columns: COLS of either half
     const int trow = cr * G8_XR + q * 32 + lane;
-    const int n_blocks = (Nout + G8_BLOCK - 1) / G8_BLOCK;
-    const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + g * (ACC / 2);
-    // accumulator columns 32 c, ... of the thread: a quarter of the tile's first half, then of its second
-    auto column_of = [](int c) { return c < ACC / 64 ? c * 32 : WR / 2 + (c - ACC / 64) * 32; };
-    // first output column of the thread's quarter of the tile's first half
-    auto col_of = [&](const Tile8& tile) { return tile.cb * tile_cols + g * (ACC / 2); };
-    // Scales: every thread copies its row's, two lanes the weights' two, into slots of the warp's own,
-    // G8_AHEAD k blocks before they are used (across tiles), asynchronously and without registers.
-    float (*slots)[G8_SLOT] = s_scale[warp - 4];
-    Tile8 ptile;
-    int pt = unit, pkb = 0, pcursor = 0, ahead = 0;
-    const float *px = nullptr, *pw = nullptr;
-    auto enter = [&]() {  // the scales of tile pt
-      ptile = locate_tile8<S::BM>(pt, pcursor, s_tile_start, s_begin, s_end);
-      px = args.xscale + ptile.row0 + (trow < ptile.nvalid ? trow : 0);
-      const int col = col_of(ptile);
-      const int nb = swiglu ? (lane & 1) * n_blocks + min(col / G8_BLOCK, n_blocks - 1)
-                            : min((col + (lane & 1) * (WR / 2)) / G8_BLOCK, n_blocks - 1);
-      pw = args.wscale + ((size_t)ptile.e * (swiglu ? 2 : 1) * n_blocks + nb) * k_blocks;
-    };
-    auto prefetch = [&]() {
-      if (pt < total_tiles) {
-        float* slot = slots[ahead & (G8_SLOTS - 1)];
-        cp_async_4(slot + lane, px);
-        if (lane < 2) cp_async_4(slot + 32 + lane, pw);
-        px += args.rows, ++pw;
-        if (++pkb == k_blocks) {
-          pkb = 0, pt += units;
-          if (pt < total_tiles) enter();
-        }
-      }
-      ++ahead;
-      cp_async_commit();
-    };
-    if (pt < total_tiles) enter();
-    for (int i = 0; i < G8_AHEAD; ++i) prefetch();
+    const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + g * S::COLS;
     int it = 0, cursor = 0;
     bool alive = true;
     for (int t = unit; t < total_tiles; t += units) {
-      const Tile8 tile = locate_tile8<S::BM>(t, cursor, s_tile_start, s_begin, s_end);
+      const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
       const bool busy = cr * G8_XR + q * 32 < tile.nvalid;  // the warp has rows of this tile
-      const bool valid = trow < tile.nvalid;
-      const int row = tile.row0 + trow, col = col_of(tile);
-      uint64_t acc[ACC / 2];
+      uint64_t acc[2][S::COLS / 2];
 #pragma unroll
-      for (int i = 0; i < ACC / 2; ++i) acc[i] = 0;
-      // Waits for the partial product of k block `it`. A warp that gave up goes on without waiting.
-      auto open = [&]() {
-        if (alive && !mbar_wait(&part_full[it & 1], (it >> 1) & 1, wait_ns)) {
+      for (int j = 0; j < S::COLS / 2; ++j) acc[0][j] = acc[1][j] = 0;
+#pragma unroll 1
+      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+        const int buf = it & 1;
+        // (a warp that gave up goes on without waiting)
+        if (alive && !mbar_wait(&part_full[buf], (it >> 1) & 1, wait_ns)) {
           *status = DS_TIMEOUT_MMA;
           alive = false;
         }
         __syncwarp();
         tc_fence_after_sync();
-      };
-      // All of it is in registers: the buffer may be overwritten.
-      auto close = [&]() {
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR) arrive_leader(cluster_map(&part_empty[it & 1], 0));
-          else mbar_arrive(&part_empty[it & 1]);
-        }
-      };
-      if (!busy) {
-        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-          prefetch();
-          open();
+        // All of the partial product is in registers: its buffer may be overwritten. The loads were
+        // the whole warp's, so one lane's word is enough.
+        auto close = [&]() {
+          tc_fence_before_sync();
+          if (elect_one()) {
+            if (PAIR) arrive_leader(cluster_map(&part_empty[buf], 0));
+            else mbar_arrive(&part_empty[buf]);
+          }
+          __syncwarp();
+        };
+        if (busy) {
+          const uint32_t from = taddr + buf * WR;
+          const float2 f = s_scale[it & (G8_SLOTS - 1)][q * 32 + lane];
+          const uint64_t f0 = twice(f.x), f1 = twice(f.y);
+          constexpr int LOADS = 2 * S::COLS / 16, PER = S::COLS / 16;  // of 16 columns: in all, and per half
+#pragma unroll
+          for (int c = 0; c < LOADS; ++c) {
+            uint32_t v[16];
+            tmem_get_x16(from + (c / PER) * (WR / 2) + (c % PER) * 16, v);
+            if (c + 1 == LOADS) close();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) fma2(acc[c / PER][(c % PER) * 8 + j], v[2 * j], v[2 * j + 1], c < PER ? f0 : f1);
+          }
+        } else {
           close();
         }
-        continue;
       }
-      uint32_t v[2][32];
-      open();
-      tmem_ld_x32(taddr + (it & 1) * WR + column_of(0), v[0]);
-#pragma unroll 1
-      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-        prefetch();
-        cp_async_wait<G8_AHEAD>();
-        __syncwarp();
-        const float* slot = slots[it & (G8_SLOTS - 1)];
-        const float x = slot[lane];
-        const uint64_t f0 = twice(x * slot[32]), f1 = twice(x * slot[33]);
-        const uint32_t from = taddr + (it & 1) * WR;
-#pragma unroll
-        for (int c = 0; c < ACC / 32; ++c) {
-          tmem_ld_wait_x32(v[c & 1]);
-          if (c + 1 < ACC / 32) {
-            tmem_ld_x32(from + column_of(c + 1), v[(c + 1) & 1]);
-          } else {  // the next block's first columns are on their way during the last multiply-adds
-            close();
-            if (kb + 1 < k_blocks) {
-              ++it;
-              open();
-              tmem_ld_x32(taddr + (it & 1) * WR + column_of(0), v[0]);
-              --it;
-            }
-          }
-          const uint64_t f = c < ACC / 64 ? f0 : f1;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) fma2(acc[c * 16 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], f);
-        }
-      }
+      const bool valid = trow < tile.nvalid;
+      const int row = tile.row0 + trow, col = tile.cb * tile_cols + g * S::COLS;
       if (!alive || !valid) continue;
       T* dst = static_cast<T*>(args.C) + (size_t)row * Nout + col;
       const float s = args.scale ? Elem<T>::to_f(static_cast<const T*>(args.scale)[row]) : 1.f;
@@ -489,8 +487,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
         uint32_t o[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const T lo = Elem<T>::from_f(f[2 * j]), hi = Elem<T>::from_f(f[2 * j + 1]);
-          o[j] = (uint32_t) reinterpret_cast<const uint16_t&>(lo) | ((uint32_t) reinterpret_cast<const uint16_t&>(hi) << 16);
+          o[j] = pack16<T>(f[2 * j], f[2 * j + 1]);
         }
         if (wide && col + c + 16 <= Nout) {
           st_global_32(dst + c, o);
@@ -499,29 +496,28 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
           if (col + c + 8 < Nout) *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(o[4], o[5], o[6], o[7]);
         }
       };
-      if (swiglu) {
+      if constexpr (SWIGLU) {
 #pragma unroll
-        for (int c = 0; c < ACC / 2; c += VALUES) {
+        for (int c = 0; c < S::COLS; c += VALUES) {
           float f[VALUES];
 #pragma unroll
           for (int j = 0; j < VALUES / 2; ++j) {
-            const float2 gate = both(acc[c / 2 + j]), up = both(acc[ACC / 4 + c / 2 + j]);
-            f[2 * j] = swiglu32(gate.x, up.x);
-            f[2 * j + 1] = swiglu32(gate.y, up.y);
+            const float2 gate = both(acc[0][c / 2 + j]), up = both(acc[1][c / 2 + j]);
+            const float2 o = swiglu32(gate, up);
+            f[2 * j] = o.x, f[2 * j + 1] = o.y;
           }
           store16(c, f);
         }
       } else {
 #pragma unroll
-        for (int c = 0; c < ACC; c += VALUES) {
+        for (int c = 0; c < 2 * S::COLS; c += VALUES) {
           float f[VALUES];
 #pragma unroll
           for (int j = 0; j < VALUES / 2; ++j) {
-            const float2 a = both(acc[c / 2 + j]);
-            f[2 * j] = a.x * s;
-            f[2 * j + 1] = a.y * s;
+            const float2 a = both(acc[c / S::COLS][c % S::COLS / 2 + j]);
+            f[2 * j] = a.x * s, f[2 * j + 1] = a.y * s;
           }
-          store16(c < ACC / 2 ? c : WR / 2 + c - ACC / 2, f);
+          store16(c < S::COLS ? c : WR / 2 + c - S::COLS, f);
         }
       }
     }
@@ -539,13 +535,13 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm8_kernel(const __grid_const
 
 // ---- host side ------------------------------------------------------------------------------
 // How many blocks (pairs: clusters of two) fit the device at once; asked once per kernel and device.
-template <typename T, int WR, bool PAIR> static int units8(int sms, int* out) {
+template <typename T, int WR, bool PAIR, bool SWIGLU> static int units8(int sms, int* out) {
   static std::atomic<int> cached[MAX_DEVICES];
   int dev = 0;
   SY_CUDA(cudaGetDevice(&dev));
   int units = cached[dev].load(std::memory_order_acquire);
   if (!units) {
-    auto kern = gemm8_kernel<T, WR, PAIR>;
+    auto kern = gemm8_kernel<T, WR, PAIR, SWIGLU>;
     SY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G8_SMEM));
     if (Shape8<WR, PAIR>::SPLIT_REGS) {
       // the promoters' register request waits for ever if the block was launched with fewer
@@ -557,7 +553,7 @@ template <typename T, int WR, bool PAIR> static int units8(int sms, int* out) {
     if (PAIR) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(sms & ~1);
-      cfg.blockDim = dim3(G8_THREADS);
+      cfg.blockDim = dim3(Shape8<WR, PAIR>::THREADS);
       cfg.dynamicSmemBytes = G8_SMEM;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -570,7 +566,7 @@ template <typename T, int WR, bool PAIR> static int units8(int sms, int* out) {
       if (units > sms / 2) units = sms / 2;
     } else {
       int per_sm = 0;
-      SY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, G8_THREADS, G8_SMEM));
+      SY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, Shape8<WR, PAIR>::THREADS, G8_SMEM));
       units = per_sm >= 1 ? sms : 0;
     }
     if (units < 1) return fail(SY_ERR_CUDA, "grouped_gemm_fp8: no block of the kernel fits on this device");
@@ -580,30 +576,31 @@ template <typename T, int WR, bool PAIR> static int units8(int sms, int* out) {
   return SY_OK;
 }
 
-template <typename T, int WR, bool PAIR>
+template <typename T, int WR, bool PAIR, bool SWIGLU>
 static int launch8(Gemm8Args a, const void* x, const void* w, cudaStream_t stream) {
   using S = Shape8<WR, PAIR>;
   int sms = 0, units = 0;
   int rc = device_sm_count(&sms);
   if (rc != SY_OK) return rc;
-  rc = units8<T, WR, PAIR>(sms, &units);
+  rc = units8<T, WR, PAIR, SWIGLU>(sms, &units);
   if (rc != SY_OK) return rc;
-  const uint64_t w_rows = (uint64_t)a.experts * (a.swiglu ? 2 : 1) * a.Nout;
+  const uint64_t w_rows = (uint64_t)a.experts * (SWIGLU ? 2 : 1) * a.Nout;
   rc = tensor_map_2d(&a.wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, w_rows, (uint64_t)a.K, S::WBOX, G8_BLOCK);
   if (rc != SY_OK) return rc;
   rc = tensor_map_2d(&a.xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XR, G8_BLOCK);
   if (rc != SY_OK) return rc;
   rc = tensor_map_2d(&a.xfew, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XFEW, G8_BLOCK);
   if (rc != SY_OK) return rc;
-  auto kern = gemm8_kernel<T, WR, PAIR>;
-  if (PAIR) return launch_cluster_kernel(kern, 2, 2 * units, G8_THREADS, G8_SMEM, stream, "grouped_gemm_fp8 launch", a);
-  return launch_kernel(kern, units, G8_THREADS, G8_SMEM, stream, "grouped_gemm_fp8 launch", a);
+  auto kern = gemm8_kernel<T, WR, PAIR, SWIGLU>;
+  if (PAIR) return launch_cluster_kernel(kern, 2, 2 * units, S::THREADS, G8_SMEM, stream, "grouped_gemm_fp8 launch", a);
+  return launch_kernel(kern, units, S::THREADS, G8_SMEM, stream, "grouped_gemm_fp8 launch", a);
 }
 
-template <typename T> static int dispatch8(const Gemm8Args& a, int tile, const void* x, const void* w, cudaStream_t s) {
-  return tile == 1 ? launch8<T, 128, false>(a, x, w, s)
-         : tile == 2 ? launch8<T, 256, false>(a, x, w, s)
-                     : launch8<T, 256, true>(a, x, w, s);
+template <typename T, bool SWIGLU>
+static int dispatch8(const Gemm8Args& a, int tile, const void* x, const void* w, cudaStream_t s) {
+  return tile == 1   ? launch8<T, 128, false, SWIGLU>(a, x, w, s)
+         : tile == 2 ? launch8<T, 256, false, SWIGLU>(a, x, w, s)
+                     : launch8<T, 256, true, SWIGLU>(a, x, w, s);
 }
 
 }  // namespace sy
@@ -635,11 +632,11 @@ extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const vo
   a.rows = rows;
   a.Nout = n_out;
   a.K = k_dim;
-  a.swiglu = swiglu != 0;
   a.status = device_status_word();
   if (!a.status) return SY_ERR_CUDA;
   a.wait_ns = wait_limit_ns();
   if (tile == 0) tile = rows <= 64LL * n_experts ? 1 : rows < 256LL * n_experts ? 2 : 3;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == SY_DTYPE_F16 ? dispatch8<__half>(a, tile, x, w, s) : dispatch8<__nv_bfloat16>(a, tile, x, w, s);
+  if (dtype == SY_DTYPE_F16) return swiglu ? dispatch8<__half, true>(a, tile, x, w, s) : dispatch8<__half, false>(a, tile, x, w, s);
+  return swiglu ? dispatch8<__nv_bfloat16, true>(a, tile, x, w, s) : dispatch8<__nv_bfloat16, false>(a, tile, x, w, s);
 }
