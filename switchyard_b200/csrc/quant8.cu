@@ -2,12 +2,18 @@
 // activations, 128 x 128 for weights.
 //
 // With m the largest magnitude of a block (at least 2^-96, so that a block of zeros has a finite
-// scale) the stored values are scale = m / 448 and q = round(448 x / m), both from a correctly
-// rounded division. 448 = 7 * 64, so 448 x is exact for 16-bit x, and a quotient that lies midway
-// between two e4m3 values comes out exactly midway and rounds to even; a multiplication by 1/m
-// would send about one value in a few thousand to the other neighbour. Both sides of the division
-// carry a factor 2^-16 so that no finite float32 overflows. A NaN makes its block's scale NaN, an
-// infinity makes it infinite: the products that use the block are then NaN, as in the input.
+// scale) the stored values are scale = m / 448 and q = e4m3(448 x / m): the correctly rounded
+// quotient, then the nearest e4m3 value, ties to even. 448 = 7 * 64, so 448 x is exact for 16-bit
+// x, and a quotient that lies midway between two e4m3 values comes out exactly midway; one product
+// with 1/m sends about one value in a thousand of bf16 data to the other neighbour.
+// A division per value is what the kernels would spend most of their time on (245 us for the
+// benchmark's gate and up projections, with two thirds of the issue slots busy). So the value is
+// bracketed by two products with 448/m, one a little small, one a little large (2^-21: more than
+// the four roundings between a product and the quotient can make). Rounding is monotone: where
+// both give the same e4m3 value it is the quotient's, and only where they differ, around the
+// midpoints, the division decides.
+// A NaN makes its block's scale NaN, an infinity makes it infinite: the products that use the block
+// are then NaN, as in the input.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -17,60 +23,98 @@ namespace sy {
 
 constexpr int Q8_BLOCK = 128;
 constexpr int Q8_THREADS = 256;
+constexpr int Q8_LANES = Q8_BLOCK / 16;  // threads that share a row of a block, 16 columns each
 constexpr float Q8_TOP = 448.f;
 
-// 8 consecutive elements as floats (16 or 32 bytes; p is 16-byte aligned).
-template <typename T> struct Eight {
-  uint4 v;
-  __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void zero() { v = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ void get(float (&f)[8]) const { unpack8<T>(v, f); }
-};
-template <> struct Eight<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = __ldg(reinterpret_cast<const float4*>(p));
-    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+// 16 consecutive elements (32 or 64 bytes from a 16-byte aligned address), as pairs of floats.
+template <typename T> struct Sixteen {
+  uint4 v[2];
+  __device__ __forceinline__ void load(const T* p) {
+    v[0] = __ldg(reinterpret_cast<const uint4*>(p));
+    v[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
   }
-  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  __device__ __forceinline__ void zero() { v[0] = v[1] = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ uint32_t word(int i) const {
+    const uint4& q = v[i >> 2];
+    return (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
   }
-};
-
-// Largest magnitude as a bit pattern: orders like the magnitude, infinities above every finite
-// value and NaNs above those, so that a maximum of integers keeps them.
-template <typename T> __device__ __forceinline__ uint32_t magnitude8(const Eight<T>& e) {
-  float f[8];
-  e.get(f);
-  uint32_t m = 0;
+  __device__ __forceinline__ float2 pair(int i) const { return Elem<T>::pair_to_f2(word(i)); }
+  // The largest magnitude's float32 bits. Bit patterns without their sign order like magnitudes,
+  // infinities above every finite value and NaNs above those.
+  __device__ __forceinline__ uint32_t magnitude() const {
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
-  return m;
-}
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, word(i) & 0x7fff7fffu);
+    const float2 f = Elem<T>::pair_to_f2(m);
+    return max(__float_as_uint(f.x), __float_as_uint(f.y));
+  }
+};
+template <> struct Sixteen<float> {
+  float4 v[4];
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __ldg(reinterpret_cast<const float4*>(p) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    return i & 1 ? make_float2(v[i >> 1].z, v[i >> 1].w) : make_float2(v[i >> 1].x, v[i >> 1].y);
+  }
+  __device__ __forceinline__ uint32_t magnitude() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = pair(i);
+      m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    }
+    return m;
+  }
+};
 
 struct BlockScale {
-  float scale, den;  // m / 448, and m * 2^-16
+  float scale, den, low, high;  // m / 448, m * 2^-16, and 448 / m bracketed
   __device__ __forceinline__ explicit BlockScale(uint32_t magnitude) {
     const float m = __uint_as_float(max(magnitude, 0x0f800000u));  // 2^-96
     scale = m / Q8_TOP;
     den = m * 0x1p-16f;
+    const float inv = Q8_TOP / m;
+    low = inv * (1.f - 0x1p-21f), high = inv * (1.f + 0x1p-21f);
   }
 };
 
-template <typename T> __device__ __forceinline__ uint2 quantize8(const Eight<T>& e, float den) {
-  float f[8];
-  e.get(f);
-  uint32_t r[4];
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// x * f for two float32 values at once.
+__device__ __forceinline__ float2 scaled(float2 x, float f) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %4};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(f));
+  return r;
+}
+
+template <typename T> __device__ __forceinline__ uint4 quantize16(const Sixteen<T>& e, const BlockScale& s) {
+  uint32_t r[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] * (Q8_TOP * 0x1p-16f) / den, f[2 * i + 1] * (Q8_TOP * 0x1p-16f) / den),
-                                    __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(r[0] | (r[1] << 16), r[2] | (r[3] << 16));
+  for (int i = 0; i < 8; ++i) {
+    const float2 x = e.pair(i), l = scaled(x, s.low), h = scaled(x, s.high);
+    r[i] = e4m3_pair(l.x, l.y);
+    if (r[i] != e4m3_pair(h.x, h.y))  // (both sides carry 2^-16: no finite value overflows)
+      r[i] = e4m3_pair(x.x * (Q8_TOP * 0x1p-16f) / s.den, x.y * (Q8_TOP * 0x1p-16f) / s.den);
+  }
+  return make_uint4(r[0] | (r[1] << 16), r[2] | (r[3] << 16), r[4] | (r[5] << 16), r[6] | (r[7] << 16));
 }
 
 // A token's row is quantised once and stored at its k places in expert order (pos_of), or at its
-// own place (pos_of absent, k = 1). Sixteen lanes share a block of 128 columns, eight each.
+// own place (pos_of absent, k = 1).
 // Scales are [blocks][rows]: what a tile of the product reads for one block is contiguous.
 template <typename T>
 __global__ void __launch_bounds__(Q8_THREADS)
@@ -84,26 +128,28 @@ quantize_rows_kernel(const T* __restrict__ x, const int* __restrict__ pos_of, co
   int pos[ROWS_MAX_K];
 #pragma unroll
   for (int j = 0; j < ROWS_MAX_K; ++j) pos[j] = j >= k ? -1 : pos_of ? pos_of[(size_t)t * k + j] : t;
-  for (int c0 = 0; c0 < blocks * 16; c0 += lanes) {
-    const int c = c0 + lane, col = c * 8;
-    Eight<T> e;
+  for (int c0 = 0; c0 < blocks * Q8_LANES; c0 += lanes) {
+    const int c = c0 + lane, col = c * 16;
+    Sixteen<T> e;
     if (col < H) e.load(x + (size_t)t * H + col);
     else e.zero();
-    uint32_t mag = magnitude8<T>(e);
+    uint32_t mag = e.magnitude();
 #pragma unroll
-    for (int o = 8; o; o >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, o));
+    for (int o = Q8_LANES / 2; o; o >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, o));
     const BlockScale s(mag);
-    const uint2 v = quantize8<T>(e, s.den);
+    const uint4 v = quantize16<T>(e, s);
+    if (col < H) {
 #pragma unroll
-    for (int j = 0; j < ROWS_MAX_K; ++j)
-      if (pos[j] >= 0 && pos[j] < m) {
-        if (col < H) *reinterpret_cast<uint2*>(q + (size_t)pos[j] * H + col) = v;
-        if ((c & 15) == 0 && col < H) scale[(size_t)(c >> 4) * m + pos[j]] = s.scale;
-      }
+      for (int j = 0; j < ROWS_MAX_K; ++j)
+        if (pos[j] >= 0 && pos[j] < m) {
+          *reinterpret_cast<uint4*>(q + (size_t)pos[j] * H + col) = v;
+          if (c % Q8_LANES == 0) scale[(size_t)(c / Q8_LANES) * m + pos[j]] = s.scale;
+        }
+    }
   }
   if (rows_used)
     for (int r = max(t * k, *rows_used); r < (t + 1) * k; ++r) {  // rows without a choice
-      for (int c = lane; c * 8 < H; c += lanes) *reinterpret_cast<uint2*>(q + (size_t)r * H + c * 8) = make_uint2(0u, 0u);
+      for (int c = lane; c * 16 < H; c += lanes) *reinterpret_cast<uint4*>(q + (size_t)r * H + c * 16) = make_uint4(0u, 0u, 0u, 0u);
       for (int b = lane; b < blocks; b += lanes) scale[(size_t)b * m + r] = 0.f;
     }
 }
@@ -113,23 +159,23 @@ quantize_rows_kernel(const T* __restrict__ x, const int* __restrict__ pos_of, co
 template <typename T>
 __global__ void __launch_bounds__(Q8_THREADS)
 quantize_weight_kernel(const T* __restrict__ w, int N, int K, uint8_t* __restrict__ q, float* __restrict__ scale) {
-  constexpr int STEP = Q8_THREADS / 16, EACH = Q8_BLOCK / STEP;
+  constexpr int STEP = Q8_THREADS / Q8_LANES, EACH = Q8_BLOCK / STEP;
   __shared__ uint32_t s_mag[Q8_THREADS / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int kb = blockIdx.x, nb = blockIdx.y;
   const size_t mat = blockIdx.z;
-  const int col = kb * Q8_BLOCK + (threadIdx.x & 15) * 8, row0 = nb * Q8_BLOCK + (threadIdx.x >> 4);
-  Eight<T> e[EACH];
-  uint32_t mag = 0;
+  const int col = kb * Q8_BLOCK + (threadIdx.x % Q8_LANES) * 16, row0 = nb * Q8_BLOCK + threadIdx.x / Q8_LANES;
+  Sixteen<T> e[EACH];
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int row = row0 + i * STEP;
     if (row < N && col < K) e[i].load(w + (mat * N + row) * K + col);
     else e[i].zero();
   }
+  uint32_t mag = 0;
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) mag = max(mag, magnitude8<T>(e[i]));
+  for (int i = 0; i < EACH; ++i) mag = max(mag, e[i].magnitude());
   mag = __reduce_max_sync(0xffffffffu, mag);
   if ((threadIdx.x & 31) == 0) s_mag[threadIdx.x >> 5] = mag;
   __syncthreads();
@@ -140,7 +186,7 @@ quantize_weight_kernel(const T* __restrict__ w, int N, int K, uint8_t* __restric
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int row = row0 + i * STEP;
-    if (row < N && col < K) *reinterpret_cast<uint2*>(q + (mat * N + row) * K + col) = quantize8<T>(e[i], s.den);
+    if (row < N && col < K) *reinterpret_cast<uint4*>(q + (mat * N + row) * K + col) = quantize16<T>(e[i], s);
   }
 }
 
@@ -148,7 +194,7 @@ template <typename T>
 static int quantize_rows_launch(const void* x, const int32_t* pos_of, const int32_t* used, int n_tokens, int k, int H,
                                 void* q, float* scale, cudaStream_t stream) {
   int lanes = 32;
-  while (lanes * 8 < H && lanes < Q8_THREADS) lanes *= 2;
+  while (lanes * 16 < H && lanes < Q8_THREADS) lanes *= 2;
   const int tokens = Q8_THREADS / lanes;
   return launch_kernel(quantize_rows_kernel<T>, (n_tokens + tokens - 1) / tokens, Q8_THREADS, 0, stream,
                        "quantize_rows launch", static_cast<const T*>(x), pos_of, used, n_tokens, k, H, lanes,
