@@ -12,7 +12,7 @@
 
 namespace sy {
 
-constexpr int ROWS_THREADS = 256;
+constexpr int ROWS_THREADS = 128;  // small blocks that come and go: 256 took 7 % longer for the gradient
 
 // Which token a thread works on, and where in its row: `lanes` threads (a multiple of 32) share a
 // token, ROWS_THREADS / lanes tokens share a block.
@@ -101,52 +101,65 @@ unpermute_rows_kernel(const T* __restrict__ y, const W* __restrict__ w, const in
 // float32 over a thread's columns, then over the lanes, then over the warps of the token, always
 // in the same order.
 template <typename T, typename W>
-__global__ void __launch_bounds__(ROWS_THREADS)
+__global__ void __launch_bounds__(ROWS_THREADS, 8)
 unpermute_rows_grad_kernel(const T* __restrict__ dout, const T* __restrict__ y, const W* __restrict__ w,
                            const int* __restrict__ pos_of, const int* __restrict__ rows_used, int n_tokens, int k,
                            int vecs, int lanes, T* __restrict__ dy, W* __restrict__ dw) {
-  constexpr int N = RowVec<T>::N;
+  constexpr int N = RowVec<T>::N, AT_ONCE = 4;  // rows whose loads are in flight together
+  __shared__ int s_pos[ROWS_THREADS / 32][ROWS_MAX_K];
+  __shared__ float s_w[ROWS_THREADS / 32][ROWS_MAX_K];
   __shared__ float s_dot[ROWS_THREADS / 32][ROWS_MAX_K];
   pdl_launch_dependents();
   pdl_wait();
   const int slot = threadIdx.x / lanes, lane = threadIdx.x % lanes;
   const int t = blockIdx.x * (ROWS_THREADS / lanes) + slot;
   const int m = n_tokens * k;
-  int pos[ROWS_MAX_K];
-  float wj[ROWS_MAX_K], dot[ROWS_MAX_K];
-#pragma unroll
-  for (int j = 0; j < ROWS_MAX_K; ++j) {
-    pos[j] = -1, wj[j] = 1.f, dot[j] = 0.f;
-    if (t < n_tokens && j < k) {
-      const int p = pos_of[(size_t)t * k + j];
-      pos[j] = p >= 0 && p < m ? p : -1;
-      if (w) wj[j] = to_float(w[(size_t)t * k + j]);
+  if (lane < ROWS_MAX_K) {
+    int p = -1;
+    float f = 1.f;
+    if (t < n_tokens && lane < k) {
+      p = pos_of[(size_t)t * k + lane];
+      if (p >= m) p = -1;
+      if (w) f = to_float(w[(size_t)t * k + lane]);
     }
+    s_pos[slot][lane] = p;
+    s_w[slot][lane] = f;
   }
+  __syncthreads();
+  float dot[ROWS_MAX_K];
+#pragma unroll
+  for (int j = 0; j < ROWS_MAX_K; ++j) dot[j] = 0.f;
   if (t < n_tokens) {
     for (int c = lane; c < vecs; c += lanes) {
-      float g[N];
-      RowVec<T>::unpack(__ldg(reinterpret_cast<const uint4*>(dout) + (size_t)t * vecs + c), g);
-      uint4 v[ROWS_MAX_K];
-      if (dw) {
+      const uint4 d = __ldg(reinterpret_cast<const uint4*>(dout) + (size_t)t * vecs + c);
 #pragma unroll
-        for (int j = 0; j < ROWS_MAX_K; ++j)
-          if (pos[j] >= 0) v[j] = __ldg(reinterpret_cast<const uint4*>(y) + (size_t)pos[j] * vecs + c);
-      }
+      for (int j0 = 0; j0 < ROWS_MAX_K; j0 += AT_ONCE) {
+        if (j0 >= k) break;
+        int pos[AT_ONCE];
+        uint4 v[AT_ONCE];
 #pragma unroll
-      for (int j = 0; j < ROWS_MAX_K; ++j) {
-        if (pos[j] < 0) continue;
-        if (dy) {
-          float r[N];
-#pragma unroll
-          for (int q = 0; q < N; ++q) r[q] = wj[j] * g[q];
-          reinterpret_cast<uint4*>(dy)[(size_t)pos[j] * vecs + c] = RowVec<T>::pack(r);
+        for (int i = 0; i < AT_ONCE; ++i) {
+          pos[i] = s_pos[slot][j0 + i];
+          if (dw && pos[i] >= 0) v[i] = __ldg(reinterpret_cast<const uint4*>(y) + (size_t)pos[i] * vecs + c);
         }
-        if (dw) {
-          float f[N];
-          RowVec<T>::unpack(v[j], f);
+        float g[N];
+        RowVec<T>::unpack(d, g);
 #pragma unroll
-          for (int q = 0; q < N; ++q) dot[j] = fmaf(g[q], f[q], dot[j]);
+        for (int i = 0; i < AT_ONCE; ++i) {
+          if (pos[i] < 0) continue;
+          if (dy) {
+            const float wj = s_w[slot][j0 + i];
+            float r[N];
+#pragma unroll
+            for (int q = 0; q < N; ++q) r[q] = wj * g[q];
+            reinterpret_cast<uint4*>(dy)[(size_t)pos[i] * vecs + c] = RowVec<T>::pack(r);
+          }
+          if (dw) {
+            float f[N];
+            RowVec<T>::unpack(v[i], f);
+#pragma unroll
+            for (int q = 0; q < N; ++q) dot[j0 + i] = fmaf(g[q], f[q], dot[j0 + i]);
+          }
         }
       }
     }
