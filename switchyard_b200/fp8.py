@@ -50,8 +50,8 @@ class Weight8(NamedTuple):
         return (self.q.float() * s.reshape(E, N, K)).to(dtype)
 
 
-def _no_grad(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad(name, t):
+    if t is not None and t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 

@@ -58,28 +58,30 @@ def _check(t, name):
     return t
 
 
-def _check_places(pos_of, offsets, like, name):
-    """(tokens, top_k) of a plan's tensors, which must be on the rows' device."""
-    if pos_of.dim() != 2 or pos_of.dtype != torch.int32 or pos_of.device != like.device:
-        raise RuntimeError(f"{name}: pos_of must be int32 [tokens, top_k] on the rows' device")
-    _check(pos_of, "pos_of")
-    if offsets is not None:
-        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.device != like.device:
-            raise RuntimeError(f"{name}: offsets must be int32 [experts + 1] on the rows' device")
-        _check(offsets, "offsets")
+def _on_device(t, name, what="x"):
+    """Index of the device of a contiguous CUDA tensor."""
+    dev = t.get_device()
+    if dev < 0 or not t.is_contiguous():
+        raise RuntimeError(f"{name}: {what} must be a contiguous CUDA tensor")
+    return dev
+
+
+def _check_places(pos_of, offsets, dev, name):
+    """(tokens, top_k) of a plan's tensors, which must be on device `dev`."""
+    if pos_of.dtype is not torch.int32 or pos_of.dim() != 2 or pos_of.get_device() != dev or not pos_of.is_contiguous():
+        raise RuntimeError(f"{name}: pos_of must be contiguous int32 [tokens, top_k] on the rows' CUDA device")
+    if offsets is not None and (offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.get_device() != dev or
+                                not offsets.is_contiguous()):
+        raise RuntimeError(f"{name}: offsets must be contiguous int32 [experts + 1] on the rows' CUDA device")
     return pos_of.shape
 
 
-def _check_weighted(y, w, N, k, name):
-    """Type codes of y [N*k, H] and its weights [N, k] (None: the rows' code)."""
-    code = _row_code(_check(y, "y"), name)
-    if y.dim() != 2 or y.shape[0] != N * k:
-        raise RuntimeError(f"{name}: y must be [{N * k}, hidden], got {list(y.shape)}")
-    if w is None:
-        return code, code
-    if w.shape != (N, k) or w.dtype not in (y.dtype, torch.float32) or w.device != y.device:
-        raise RuntimeError(f"{name}: w must be [{N}, {k}], float32 or of the rows' dtype, on their device")
-    return code, _row_code(_check(w, "w"), name)
+def _check_weights(w, rows, N, k, dev, name):
+    """Type code of the weights [N, k] of rows in dtype `rows`."""
+    if (w.dtype is not rows and w.dtype is not torch.float32) or w.shape != (N, k) or w.get_device() != dev or \
+            not w.is_contiguous():
+        raise RuntimeError(f"{name}: w must be contiguous [{N}, {k}], float32 or of the rows' dtype, on their CUDA device")
+    return _row_code(w, name)
 
 
 def _ptr(t):
@@ -91,16 +93,19 @@ class _Device:
 
     __slots__ = ("dev", "prev")
 
-    def __init__(self, dev):
-        self.dev = dev.index if dev.index is not None else torch.cuda.current_device()
+    def __init__(self, dev):  # a torch.device, or the index of one
+        if type(dev) is not int:
+            dev = dev.index if dev.index is not None else torch.cuda.current_device()
+        self.dev = dev
         self.prev = -1
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
+        # the binding's own look-ups: the public ones build a Stream object, 1.2 us of a 12 us call
+        cur = torch._C._cuda_getDevice()
         if cur != self.dev:
             self.prev = cur
             torch.cuda.set_device(self.dev)
-        return torch.cuda.current_stream(self.dev).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.dev)
 
     def __exit__(self, *a):
         if self.prev >= 0:
@@ -330,71 +335,75 @@ class Ext:
 
     def permute_rows(self, h, pos_of, offsets):
         """x [N*k, H] with x[pos_of[t, j]] = h[t] (rows.permute_rows adds the gradient)."""
-        N, k = _check_places(pos_of, offsets, h, "permute_rows")
+        dev, code = _on_device(h, "permute_rows", "h"), _row_code(h, "permute_rows")
+        N, k = _check_places(pos_of, offsets, dev, "permute_rows")
         if h.dim() != 2 or h.shape[0] != N:
             raise RuntimeError(f"permute_rows: h must be [{N}, hidden], got {list(h.shape)}")
-        code, H = _row_code(_check(h, "h"), "permute_rows"), h.shape[1]
-        x = torch.empty(N * k, H, dtype=h.dtype, device=h.device)
-        with _Device(h.device) as stream:
-            _lib.check(self.lib.sy_permute_rows(_ptr(h), _ptr(pos_of), _ptr(offsets), N, k, offsets.numel() - 1, H, code,
-                                                _ptr(x), stream), "permute_rows")
+        H = h.shape[1]
+        x = torch.empty((N * k, H), dtype=h.dtype, device=h.device)
+        with _Device(dev) as stream:
+            rc = self.lib.sy_permute_rows(h.data_ptr(), pos_of.data_ptr(), offsets.data_ptr(), N, k, offsets.numel() - 1, H,
+                                          code, x.data_ptr(), stream)
+        _lib.check(rc, "permute_rows")
         return x
 
     def unpermute_rows(self, y, w, pos_of):
         """out [N, H] = sum_j w[t, j] * y[pos_of[t, j]]; w None: all one (rows.unpermute_rows adds
         the gradients)."""
-        N, k = _check_places(pos_of, None, y, "unpermute_rows")
-        code, wcode = _check_weighted(y, w, N, k, "unpermute_rows")
+        dev, code = _on_device(y, "unpermute_rows", "y"), _row_code(y, "unpermute_rows")
+        N, k = _check_places(pos_of, None, dev, "unpermute_rows")
+        if y.dim() != 2 or y.shape[0] != N * k:
+            raise RuntimeError(f"unpermute_rows: y must be [{N * k}, hidden], got {list(y.shape)}")
+        wcode = code if w is None else _check_weights(w, y.dtype, N, k, dev, "unpermute_rows")
         H = y.shape[1]
-        out = torch.empty(N, H, dtype=y.dtype, device=y.device)
-        with _Device(y.device) as stream:
-            _lib.check(self.lib.sy_unpermute_rows(_ptr(y), _ptr(w), wcode, _ptr(pos_of), N, k, H, code, _ptr(out), stream),
-                       "unpermute_rows")
+        out = torch.empty((N, H), dtype=y.dtype, device=y.device)
+        with _Device(dev) as stream:
+            rc = self.lib.sy_unpermute_rows(y.data_ptr(), _ptr(w), wcode, pos_of.data_ptr(), N, k, H, code, out.data_ptr(),
+                                            stream)
+        _lib.check(rc, "unpermute_rows")
         return out
 
     def unpermute_rows_grad(self, dout, y, w, pos_of, offsets, need_dy=True, need_dw=True):
         """(dy, dw) of unpermute_rows; what is not needed is None, and y may be None without dw."""
-        N, k = _check_places(pos_of, offsets, dout, "unpermute_rows_grad")
-        code, H = _row_code(_check(dout, "dout"), "unpermute_rows_grad"), dout.shape[1]
-        if dout.shape != (N, H):
-            raise RuntimeError(f"unpermute_rows_grad: dout must be [{N}, hidden], got {list(dout.shape)}")
-        if y is not None and (y.dtype != dout.dtype or y.shape != (N * k, H) or y.device != dout.device):
-            raise RuntimeError(f"unpermute_rows_grad: y must be [{N * k}, {H}] in dout's dtype and on its device")
+        name = "unpermute_rows_grad"
+        dev, code = _on_device(dout, name, "dout"), _row_code(dout, name)
+        N, k = _check_places(pos_of, offsets, dev, name)
+        if dout.dim() != 2 or dout.shape[0] != N:
+            raise RuntimeError(f"{name}: dout must be [{N}, hidden], got {list(dout.shape)}")
+        H = dout.shape[1]
+        if y is not None and (y.dtype != dout.dtype or y.shape != (N * k, H) or _on_device(y, name, "y") != dev):
+            raise RuntimeError(f"{name}: y must be [{N * k}, {H}] in dout's dtype and on its device")
         if need_dw and (y is None or w is None):
-            raise RuntimeError("unpermute_rows_grad: the weights' gradient needs y and w")
-        wcode = code
-        if y is not None:
-            _check(y, "y")
-        if w is not None:
-            if w.shape != (N, k) or w.dtype not in (dout.dtype, torch.float32) or w.device != dout.device:
-                raise RuntimeError(f"unpermute_rows_grad: w must be [{N}, {k}], float32 or of the rows' dtype")
-            wcode = _row_code(_check(w, "w"), "unpermute_rows_grad")
-        dy = torch.empty(N * k, H, dtype=dout.dtype, device=dout.device) if need_dy else None
+            raise RuntimeError(f"{name}: the weights' gradient needs y and w")
+        wcode = code if w is None else _check_weights(w, dout.dtype, N, k, dev, name)
+        dy = torch.empty((N * k, H), dtype=dout.dtype, device=dout.device) if need_dy else None
         dw = torch.empty_like(w) if need_dw else None
-        with _Device(dout.device) as stream:
-            _lib.check(self.lib.sy_unpermute_rows_grad(_ptr(dout), _ptr(y), _ptr(w), wcode, _ptr(pos_of), _ptr(offsets), N, k,
-                                                       offsets.numel() - 1, H, code, _ptr(dy), _ptr(dw), stream),
-                       "unpermute_rows_grad")
+        with _Device(dev) as stream:
+            rc = self.lib.sy_unpermute_rows_grad(dout.data_ptr(), _ptr(y), _ptr(w), wcode, pos_of.data_ptr(),
+                                                 offsets.data_ptr(), N, k, offsets.numel() - 1, H, code, _ptr(dy), _ptr(dw),
+                                                 stream)
+        _lib.check(rc, name)
         return dy, dw
 
     def quantize_rows(self, x, pos_of=None, offsets=None):
         """(q float8_e4m3fn [rows, H], scale float32 [ceil(H/128), rows]) of x [N, H]; with pos_of and
         offsets the rows come in expert order, rows = N*k."""
+        dev, code = _on_device(x, "quantize_rows"), _row_code(x, "quantize_rows")
         if x.dim() != 2:
             raise RuntimeError(f"quantize_rows: x must be [tokens, hidden], got {list(x.shape)}")
         N, H = x.shape
-        k = 1
-        code = _row_code(_check(x, "x"), "quantize_rows")
+        k = experts = 1
         if pos_of is not None:
-            n, k = _check_places(pos_of, offsets, x, "quantize_rows")
+            n, k = _check_places(pos_of, offsets, dev, "quantize_rows")
+            experts = offsets.numel() - 1
             if n != N:
                 raise RuntimeError(f"quantize_rows: x has {N} rows, the plan {n} tokens")
-        q = torch.empty(N * k, H, dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty((H + 127) // 128, N * k, dtype=torch.float32, device=x.device)
-        with _Device(x.device) as stream:
-            _lib.check(self.lib.sy_quantize_rows(_ptr(x), _ptr(pos_of), _ptr(offsets), N, k,
-                                                 offsets.numel() - 1 if pos_of is not None else 0, H, code, _ptr(q),
-                                                 _ptr(scale), stream), "quantize_rows")
+        q = torch.empty((N * k, H), dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(((H + 127) // 128, N * k), dtype=torch.float32, device=x.device)
+        with _Device(dev) as stream:
+            rc = self.lib.sy_quantize_rows(x.data_ptr(), _ptr(pos_of), _ptr(offsets) if pos_of is not None else None, N, k,
+                                           experts, H, code, q.data_ptr(), scale.data_ptr(), stream)
+        _lib.check(rc, "quantize_rows")
         return q, scale
 
     def quantize_weight(self, w, halves=1):
@@ -414,12 +423,12 @@ class Ext:
     def grouped_gemm_fp8(self, x, x_scale, w, w_scale, offsets, swiglu, scale, dtype, tile=0):
         """The experts' product of 8-bit rows and weights (sy_grouped_gemm_fp8): C [rows, n_out]."""
         name = "grouped_gemm_fp8"
+        dev = _on_device(x, name)
         for t, what, dt, dims in ((x, "x", torch.float8_e4m3fn, 2), (x_scale, "x_scale", torch.float32, 2),
                                   (w, "w", torch.float8_e4m3fn, 3), (w_scale, "w_scale", torch.float32, 3),
                                   (offsets, "offsets", torch.int32, 1)):
-            if t.dtype != dt or t.dim() != dims or t.device != x.device:
-                raise RuntimeError(f"{name}: {what} must be {dt} with {dims} dimensions, on x's device")
-            _check(t, what)
+            if t.dtype is not dt or t.dim() != dims or t.get_device() != dev or not t.is_contiguous():
+                raise RuntimeError(f"{name}: {what} must be a contiguous CUDA tensor of {dt} with {dims} dimensions, on x's device")
         (rows, K), (E, Nfull, wk) = x.shape, w.shape
         parts = 2 if swiglu else 1
         if Nfull % parts:
@@ -430,18 +439,17 @@ class Ext:
         if w_scale.shape != (E, parts * ((n_out + 127) // 128), kb):
             raise RuntimeError(f"{name}: w_scale must be [{E}, {parts * ((n_out + 127) // 128)}, {kb}], got "
                                f"{list(w_scale.shape)}" + (" (quantise gate and up as two halves)" if swiglu else ""))
-        if dtype not in (torch.float16, torch.bfloat16):
+        if dtype is not torch.float16 and dtype is not torch.bfloat16:
             raise RuntimeError(f"{name}: the result is fp16 or bf16, not {dtype}")
-        if scale is not None and (scale.dtype != dtype or scale.shape != (rows,) or scale.device != x.device):
-            raise RuntimeError(f"{name}: scale must be [{rows}] in the result's dtype")
-        C = torch.empty(rows, n_out, dtype=dtype, device=x.device)
-        code = _lib.SY_DTYPE_F16 if dtype == torch.float16 else _lib.SY_DTYPE_BF16
-        if scale is not None:
-            _check(scale, "scale")
-        with _Device(x.device) as stream:
-            _lib.check(self.lib.sy_grouped_gemm_fp8(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(offsets), E, rows,
-                                                    n_out, K, int(bool(swiglu)), _ptr(scale), _ptr(C), code, int(tile),
-                                                    stream), name)
+        if scale is not None and (scale.dtype is not dtype or scale.shape != (rows,) or _on_device(scale, name, "scale") != dev):
+            raise RuntimeError(f"{name}: scale must be [{rows}] in the result's dtype, on x's device")
+        C = torch.empty((rows, n_out), dtype=dtype, device=x.device)
+        code = _lib.SY_DTYPE_F16 if dtype is torch.float16 else _lib.SY_DTYPE_BF16
+        with _Device(dev) as stream:
+            rc = self.lib.sy_grouped_gemm_fp8(x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+                                              offsets.data_ptr(), E, rows, n_out, K, 1 if swiglu else 0, _ptr(scale),
+                                              C.data_ptr(), code, int(tile), stream)
+        _lib.check(rc, name)
         return C
 
     def gather_rows(self, src, index, dst):

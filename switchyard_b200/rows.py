@@ -27,9 +27,16 @@ class SortPlan(NamedTuple):
     pos_of: torch.Tensor   # int32 [N, k]
 
 
+_kernels = None
+
+
 def _ext():
-    from . import kernels
-    return kernels.ext()
+    """The kernel library's calls (kernels imports this module: looked up at the first call)."""
+    global _kernels
+    if _kernels is None:
+        from . import kernels
+        _kernels = kernels
+    return _kernels.ext()
 
 
 def plan(idx, n_experts):
