@@ -7,7 +7,7 @@
 // Float32 scales cannot ride in the tensor core, so the inner sums of each block of 128 (four
 // tcgen05.mma of k = 32) go to tensor memory on their own and eight warps multiply them by the
 // two scales and add them up in float32 registers while the next block is being multiplied:
-// tensor memory holds two such partial products. A thread owns a row of the tile and a half of its
+// tensor memory holds two such partial products of 256 columns, or four of 128. A thread owns a row of the tile and a half of its
 // columns. Both factors of a step are the same for all of a thread's columns of one weight block,
 // so the promotion costs one packed multiply-add per two values.
 //
@@ -34,7 +34,9 @@ constexpr int G8_BLOCK = 128;                    // k per scale and per stage: o
 constexpr int G8_XR = 128;                       // token rows a CTA stages
 constexpr int G8_XFEW = 32;                      // token rows of the small TMA box, for tiles of at most two of them
 constexpr int G8_MAX_E = 256;
-constexpr int G8_SLOTS = 4;                      // k blocks whose scales are in shared memory
+constexpr int G8_AHEAD = 7;                      // k blocks whose scales are on their way
+constexpr int G8_SLOTS = 16;                     // k blocks whose scales are in shared memory or on their way
+constexpr int G8_SLOT = G8_XR + 8;               // floats: the rows' scales, then the weights' two
 constexpr int G8_HELPERS = 4;                    // warps before the promoters: TMA, two for MMA, scales
 constexpr int G8_RING_BYTES = 192 * 1024;
 constexpr int G8_SMEM = G8_RING_BYTES + 1024;    // room to align the ring to 1024
@@ -49,7 +51,8 @@ template <int WR, bool PAIR> struct Shape8 {
   static constexpr int X_BYTES = G8_XR * G8_BLOCK;
   static constexpr int STAGE_BYTES = X_BYTES + WRC * G8_BLOCK;
   static constexpr int STAGES = G8_RING_BYTES / STAGE_BYTES;
-  static constexpr int TMEM_COLS = 2 * WR;                // two partial products
+  static constexpr int BUFS = 512 / WR;                   // partial products: all of tensor memory
+  static constexpr int TMEM_COLS = BUFS * WR;
   static constexpr int PROMOTERS = 8;                     // warps
   static constexpr int THREADS = (G8_HELPERS + PROMOTERS) * 32;
   static constexpr int COLS = WR / 4;                     // columns a promoter thread has of either half
@@ -95,16 +98,42 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
       "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 32 lanes x 16 consecutive columns of tensor memory, and the wait for them in the same statement: the
-// registers are not to be touched before it.
-__device__ __forceinline__ void tmem_get_x16(uint32_t addr, uint32_t (&r)[16]) {
+// 32 lanes x 32 consecutive columns of tensor memory, and the wait for them in the same statement: the
+// registers are not to be touched before it. (Two loads of 16: 32 registers in a row would have to be
+// found otherwise.)
+__device__ __forceinline__ void tmem_get_32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32 + 16];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr)
       : "memory");
+}
+// 32 columns from either address.
+__device__ __forceinline__ void tmem_get_32_32(uint32_t a, uint32_t b, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64 + 16];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47}, [%65];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65 + 16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(a), "r"(b)
+      : "memory");
+}
+__device__ __forceinline__ void cp_async_4(float* dst_smem, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst_smem)), "l"(src) : "memory");
 }
 // acc += part * f for two float32 values at once. The accumulators are 64-bit values throughout, so
 // that they stay in aligned register pairs.
@@ -194,16 +223,16 @@ __device__ __forceinline__ float2 swiglu32(float2 g, float2 u) {
 template <typename T, int WR, bool PAIR, bool SWIGLU>
 __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(const __grid_constant__ Gemm8Args args) {
   using S = Shape8<WR, PAIR>;
-  constexpr int STAGES = S::STAGES;
+  constexpr int STAGES = S::STAGES, BUFS = S::BUFS;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES];
   __shared__ __align__(8) uint64_t empty_bar[STAGES];
-  __shared__ __align__(8) uint64_t part_full[2];
-  __shared__ __align__(8) uint64_t part_empty[2];
+  __shared__ __align__(8) uint64_t part_full[BUFS];
+  __shared__ __align__(8) uint64_t part_empty[BUFS];
   __shared__ uint32_t s_tmem;
   __shared__ int s_begin[G8_MAX_E], s_end[G8_MAX_E];
   __shared__ int s_tile_start[G8_MAX_E + 1];
-  __shared__ float2 s_scale[G8_SLOTS][G8_XR];  // per row: its scale times the weights', of either half
+  __shared__ float s_scale[G8_SLOTS][G8_SLOT];
 
   // (uniform to the compiler, so that the roles are too)
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -224,7 +253,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < BUFS; ++b) {
       mbar_init(&part_full[b], 2);                           // the MMAs, and this CTA's scales
       mbar_init(&part_empty[b], S::CTAS * S::PROMOTERS);  // PAIR: the leader's, for both CTAs
     }
@@ -323,7 +352,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full_bar[j % STAGES], (j / STAGES) & 1, 10000000ull);
     } else if (warp <= 2) {
       // -------------------------------------------------------------- MMA issuers (PAIR: the leader's, for both CTAs)
-      // One warp for either partial product: the k blocks in turn. A wait costs its warp 100 to 250
+      // Two warps take the k blocks in turn. A wait costs its warp 100 to 250
       // clocks even when there is nothing to wait for; with one warp for all blocks those came
       // one after another, 750 clocks a block.
       // The whole warp walks the blocks (so that descriptors and loop counters stay in uniform
@@ -332,15 +361,14 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         const uint32_t ring_lo = umma_desc_lo(smem_u32(stages));
         const uint32_t idesc = umma_idesc(0, S::BM, WR);  // format 0 is e4m3 in this kind
         const int n = total_tiles > unit ? ((total_tiles - unit + units - 1) / units) * k_blocks : 0;
-        const int buf = warp - 1;
-        const uint32_t d = tmem + buf * WR;
-        for (int it = buf; it < n; it += 2) {
-          const int s = it % STAGES;
+        for (int it = warp - 1; it < n; it += 2) {
+          const int s = it % STAGES, buf = it % BUFS;
+          const uint32_t d = tmem + buf * WR;
           if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, wait_ns)) {
             *status = DS_TIMEOUT_FULL;
             break;
           }
-          if (it >= 2 && !mbar_wait(&part_empty[buf], ((it >> 1) - 1) & 1, wait_ns)) {
+          if (it >= BUFS && !mbar_wait(&part_empty[buf], (it / BUFS - 1) & 1, wait_ns)) {
             *status = DS_TIMEOUT_TMEM;
             break;
           }
@@ -369,61 +397,57 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(args.C) + (size_t)(r < lo ? r : hi + (r - lo)) * Nout);
         for (int c = lane; c < Nout / 8; c += 32) row[c] = make_uint4(0u, 0u, 0u, 0u);
       }
-      // A lane has four of the CTA's rows.
+      // Every block's scales are copied asynchronously, G8_AHEAD blocks before their turn: the first
+      // ones come from DRAM, behind the weights. (Loads into registers are no ring: waiting for an
+      // old one waits for the young ones too, 3000 clocks a block at the start of a launch.) When they
+      // are there the block's partial product gets this warp's word, which is due only once the
+      // block before in the same partial product has had its own: by then the block before that one
+      // is promoted, so at most G8_AHEAD + 2 BUFS + 1 slots are in use.
+      static_assert(G8_AHEAD + 2 * BUFS + 1 <= G8_SLOTS, "slots");
       const int n_blocks = (Nout + G8_BLOCK - 1) / G8_BLOCK;
-      int t = unit, kb = 0, cursor = 0;
+      const int n = total_tiles > unit ? ((total_tiles - unit + units - 1) / units) * k_blocks : 0;
+      int t = unit, kb = 0, cursor = 0, mine = 0, ahead = 0;
       const float *px = nullptr, *pw = nullptr;
-      int own[4];
-      auto enter = [&]() {  // the tile of the next block
+      auto enter = [&]() {  // tile t
         const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = cr * G8_XR + lane + 32 * i;
-          own[i] = r < tile.nvalid ? r : 0;
-        }
-        px = args.xscale + tile.row0;
+        mine = min(max(tile.nvalid - cr * G8_XR, 0), G8_XR);
+        px = args.xscale + tile.row0 + cr * G8_XR + lane;
         const int col = tile.cb * tile_cols;
         const int nb = SWIGLU ? (lane & 1) * n_blocks + col / G8_BLOCK
                               : min((col + (lane & 1) * (WR / 2)) / G8_BLOCK, n_blocks - 1);
         pw = args.wscale + ((size_t)tile.e * (SWIGLU ? 2 : 1) * n_blocks + nb) * k_blocks;  // lane parity: the half
       };
-      float x[2][4], w[2];  // asked for two rounds before they are used
-      auto fetch = [&](int i) {
-        if (t >= total_tiles) return;
+      auto fetch = [&]() {
+        if (ahead < n) {
+          float* slot = s_scale[ahead % G8_SLOTS];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[i][r] = __ldg(px + own[r]);
-        w[i] = __ldg(pw);
-        px += args.rows, ++pw;
-        if (++kb == k_blocks) {
-          kb = 0, t += units;
-          if (t < total_tiles) enter();
+          for (int r = 0; r < G8_XR; r += 32)
+            if (r + lane < mine) cp_async_4(slot + r + lane, px + r);
+          if (lane < 2) cp_async_4(slot + G8_XR + lane, pw);
+          px += args.rows, ++pw;
+          if (++kb == k_blocks) {
+            kb = 0, t += units;
+            if (t < total_tiles) enter();
+          }
         }
+        ++ahead;
+        cp_async_commit();
       };
-      const int n = total_tiles > unit ? ((total_tiles - unit + units - 1) / units) * k_blocks : 0;
       if (n) enter();
-      fetch(0);
-      fetch(1);
-      bool alive = true;
-      auto round = [&](int it, int i) {
-        // Block it - 2 has been multiplied, so its predecessor in the same slot has been promoted; and
-        // this block's word cannot be taken for that one's.
-        if (it >= 2 && !mbar_wait(&part_full[i], ((it >> 1) - 1) & 1, wait_ns)) {
+      for (int i = 0; i < G8_AHEAD; ++i) fetch();
+      for (int it = 0; it < n; ++it) {
+        const int buf = it % BUFS;
+        if (it >= BUFS && !mbar_wait(&part_full[buf], (it / BUFS - 1) & 1, wait_ns)) {
           *status = DS_TIMEOUT_MMA;
-          alive = false;
-          return;
+          break;
         }
-        float2* slot = s_scale[it & (G8_SLOTS - 1)];
-        const float w0 = __shfl_sync(0xffffffffu, w[i], 0), w1 = __shfl_sync(0xffffffffu, w[i], 1);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) slot[lane + 32 * r] = make_float2(x[i][r] * w0, x[i][r] * w1);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&part_full[i]);
-        fetch(i);
-      };
-      for (int it = 0; it < n && alive; it += 2) {
-        round(it, 0);
-        if (it + 1 < n && alive) round(it + 1, 1);
+        fetch();
+        cp_async_wait<G8_AHEAD>();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&part_full[buf]);
       }
+      cp_async_wait<0>();
     }
   } else {
     // ---------------------------------------------------------------- promotion and epilogue
@@ -433,17 +457,19 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
     const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + g * S::COLS;
     int it = 0, cursor = 0;
     bool alive = true;
+    Tile8 next;
+    if (unit < total_tiles) next = locate_tile8<S::BM>(unit, cursor, E, s_tile_start, s_begin, s_end);
     for (int t = unit; t < total_tiles; t += units) {
-      const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
+      const Tile8 tile = next;
       const bool busy = cr * G8_XR + q * 32 < tile.nvalid;  // the warp has rows of this tile
       uint64_t acc[2][S::COLS / 2];
 #pragma unroll
       for (int j = 0; j < S::COLS / 2; ++j) acc[0][j] = acc[1][j] = 0;
 #pragma unroll 1
       for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-        const int buf = it & 1;
+        const int buf = it % BUFS;
         // (a warp that gave up goes on without waiting)
-        if (alive && !mbar_wait(&part_full[buf], (it >> 1) & 1, wait_ns)) {
+        if (alive && !mbar_wait(&part_full[buf], (it / BUFS) & 1, wait_ns)) {
           *status = DS_TIMEOUT_MMA;
           alive = false;
         }
@@ -461,20 +487,28 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         };
         if (busy) {
           const uint32_t from = taddr + buf * WR;
-          const float2 f = s_scale[it & (G8_SLOTS - 1)][q * 32 + lane];
-          const uint64_t f0 = twice(f.x), f1 = twice(f.y);
-          constexpr int LOADS = 2 * S::COLS / 16, PER = S::COLS / 16;  // of 16 columns: in all, and per half
+          const float* slot = s_scale[it % G8_SLOTS];
+          const float sx = slot[q * 32 + lane];
+          const uint64_t f0 = twice(sx * slot[G8_XR]), f1 = twice(sx * slot[G8_XR + 1]);
+          // as many columns at once as there are registers for: a load takes its 70 clocks either way
+          constexpr int AT_ONCE = S::COLS > 32 ? 32 : 64, GROUPS = 2 * S::COLS / AT_ONCE;
 #pragma unroll
-          for (int c = 0; c < LOADS; ++c) {
-            uint32_t v[16];
-            tmem_get_x16(from + (c / PER) * (WR / 2) + (c % PER) * 16, v);
-            if (c + 1 == LOADS) close();
+          for (int c = 0; c < GROUPS; ++c) {
+            uint32_t v[AT_ONCE];
+            if constexpr (AT_ONCE == 64) tmem_get_32_32(from, from + WR / 2, v);
+            else tmem_get_32(from + (c * 32 / S::COLS) * (WR / 2) + c * 32 % S::COLS, v);
+            if (c + 1 == GROUPS) close();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) fma2(acc[c / PER][(c % PER) * 8 + j], v[2 * j], v[2 * j + 1], c < PER ? f0 : f1);
+            for (int j = 0; j < AT_ONCE / 2; ++j) {
+              const int at = c * AT_ONCE + 2 * j;  // of the thread's columns
+              fma2(acc[at / S::COLS][at % S::COLS / 2], v[2 * j], v[2 * j + 1], at < S::COLS ? f0 : f1);
+            }
           }
         } else {
           close();
         }
+        if (kb == 0 && t + units < total_tiles)  // found while the next block is being multiplied
+          next = locate_tile8<S::BM>(t + units, cursor, E, s_tile_start, s_begin, s_end);
       }
       const bool valid = trow < tile.nvalid;
       const int row = tile.row0 + trow, col = tile.cb * tile_cols + g * S::COLS;
