@@ -36,6 +36,7 @@ constexpr int G8_XFEW = 32;                      // token rows of the small TMA 
 constexpr int G8_MAX_E = 256;
 constexpr int G8_AHEAD = 7;                      // k blocks whose scales are on their way
 constexpr int G8_SLOTS = 16;                     // k blocks whose scales are in shared memory or on their way
+constexpr int G8_OUT_PITCH = 64 + 16;             // bytes per staged row of results: 32 columns, off the banks of the next
 constexpr int G8_SLOT = G8_XR + 8;               // floats: the rows' scales, then the weights' two
 constexpr int G8_HELPERS = 4;                    // warps before the promoters: TMA, two for MMA, scales
 constexpr int G8_RING_BYTES = 192 * 1024;
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
   __shared__ int s_begin[G8_MAX_E], s_end[G8_MAX_E];
   __shared__ int s_tile_start[G8_MAX_E + 1];
   __shared__ float s_scale[G8_SLOTS][G8_SLOT];
+  __shared__ __align__(16) unsigned char s_out[S::PROMOTERS][32 * G8_OUT_PITCH];
 
   // (uniform to the compiler, so that the roles are too)
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -462,6 +464,8 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
     for (int t = unit; t < total_tiles; t += units) {
       const Tile8 tile = next;
       const bool busy = cr * G8_XR + q * 32 < tile.nvalid;  // the warp has rows of this tile
+      float row_scale = 1.f;
+      if (!SWIGLU && args.scale && trow < tile.nvalid) row_scale = Elem<T>::to_f(static_cast<const T*>(args.scale)[tile.row0 + trow]);
       uint64_t acc[2][S::COLS / 2];
 #pragma unroll
       for (int j = 0; j < S::COLS / 2; ++j) acc[0][j] = acc[1][j] = 0;
@@ -510,48 +514,47 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         if (kb == 0 && t + units < total_tiles)  // found while the next block is being multiplied
           next = locate_tile8<S::BM>(t + units, cursor, E, s_tile_start, s_begin, s_end);
       }
-      const bool valid = trow < tile.nvalid;
-      const int row = tile.row0 + trow, col = tile.cb * tile_cols + g * S::COLS;
-      if (!alive || !valid) continue;
-      T* dst = static_cast<T*>(args.C) + (size_t)row * Nout + col;
-      const float s = args.scale ? Elem<T>::to_f(static_cast<const T*>(args.scale)[row]) : 1.f;
-      const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
-      constexpr int VALUES = 16;
-      auto store16 = [&](int c, const float (&f)[VALUES]) {  // columns col + c, ...
-        uint32_t o[8];
+      alive = __all_sync(0xffffffffu, alive);
+      if (!alive || !busy) continue;
+      const int rows = tile.nvalid - (cr * G8_XR + q * 32), col = tile.cb * tile_cols + g * S::COLS;
+      T* to = static_cast<T*>(args.C) + (size_t)(tile.row0 + cr * G8_XR + q * 32) * Nout + col;
+      // Thirty-two columns from col + c on, a row per lane, to memory by way of shared memory: a store
+      // then covers eight rows of 64 bytes, where a lane's own row would make it touch 32 lines.
+      auto store32 = [&](int c, const uint32_t (&o)[16]) {
+        unsigned char* mine = s_out[warp - G8_HELPERS] + lane * G8_OUT_PITCH;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          o[j] = pack16<T>(f[2 * j], f[2 * j + 1]);
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(mine + i * 16) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        __syncwarp();
+        const int part = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + (lane >> 2);
+          const uint4 v = *reinterpret_cast<const uint4*>(s_out[warp - G8_HELPERS] + r * G8_OUT_PITCH + part * 16);
+          if (r < rows && col + c + part * 8 < Nout) *reinterpret_cast<uint4*>(to + (size_t)r * Nout + c + part * 8) = v;
         }
-        if (wide && col + c + 16 <= Nout) {
-          st_global_32(dst + c, o);
-        } else {
-          if (col + c < Nout) *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[0], o[1], o[2], o[3]);
-          if (col + c + 8 < Nout) *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(o[4], o[5], o[6], o[7]);
-        }
+        __syncwarp();
       };
       if constexpr (SWIGLU) {
 #pragma unroll
-        for (int c = 0; c < S::COLS; c += VALUES) {
-          float f[VALUES];
+        for (int c = 0; c < S::COLS; c += 32) {
+          uint32_t o[16];
 #pragma unroll
-          for (int j = 0; j < VALUES / 2; ++j) {
-            const float2 gate = both(acc[0][c / 2 + j]), up = both(acc[1][c / 2 + j]);
-            const float2 o = swiglu32(gate, up);
-            f[2 * j] = o.x, f[2 * j + 1] = o.y;
+          for (int j = 0; j < 16; ++j) {
+            const float2 v = swiglu32(both(acc[0][c / 2 + j]), both(acc[1][c / 2 + j]));
+            o[j] = pack16<T>(v.x, v.y);
           }
-          store16(c, f);
+          store32(c, o);
         }
       } else {
 #pragma unroll
-        for (int c = 0; c < 2 * S::COLS; c += VALUES) {
-          float f[VALUES];
+        for (int c = 0; c < 2 * S::COLS; c += 32) {
+          uint32_t o[16];
 #pragma unroll
-          for (int j = 0; j < VALUES / 2; ++j) {
-            const float2 a = both(acc[c / S::COLS][c % S::COLS / 2 + j]);
-            f[2 * j] = a.x * s, f[2 * j + 1] = a.y * s;
+          for (int j = 0; j < 16; ++j) {
+            const float2 v = both(acc[c / S::COLS][c % S::COLS / 2 + j]);
+            o[j] = pack16<T>(v.x * row_scale, v.y * row_scale);
           }
-          store16(c < S::COLS ? c : WR / 2 + c - S::COLS, f);
+          store32(c < S::COLS ? c : WR / 2 + c - S::COLS, o);
         }
       }
     }
