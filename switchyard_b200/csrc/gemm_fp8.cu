@@ -32,7 +32,7 @@ namespace sy {
 
 constexpr int G8_BLOCK = 128;                    // k per scale and per stage: one 128-byte swizzle atom
 constexpr int G8_XR = 128;                       // token rows a CTA stages
-constexpr int G8_XFEW = 32;                      // token rows of the small TMA box, for tiles of at most two of them
+constexpr int G8_XFEW = 32;                      // token rows of the small TMA box, for tiles with fewer rows
 constexpr int G8_MAX_E = 256;
 constexpr int G8_AHEAD = 7;                      // k blocks whose scales are on their way
 constexpr int G8_SLOTS = 16;                     // k blocks whose scales are in shared memory or on their way
@@ -313,15 +313,14 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
       bool alive = true;
       for (int t = unit; t < total_tiles && alive; t += units) {
         const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
-        // token rows: one box of 128, or one or two of 32 where the tile has no more
+        // Token rows: one box of 128 where the tile has that many, else boxes of 32 as far as there are rows.
+        // What is multiplied in the others' place is never read.
         auto rows_of = [&](int c) { return min(max(tile.nvalid - c * G8_XR, 0), G8_XR); };
-        auto x_bytes = [&](int n) {
-          return n > 2 * G8_XFEW ? S::X_BYTES : (n + G8_XFEW - 1) / G8_XFEW * (G8_XFEW * G8_BLOCK);
-        };
-        const int mine = rows_of(cr);
-        const bool few = mine <= 2 * G8_XFEW;
-        const int x_boxes = few ? (mine + G8_XFEW - 1) / G8_XFEW : 1;
-        const uint32_t bytes = WR * G8_BLOCK + x_bytes(mine) + (PAIR ? x_bytes(rows_of(cr ^ 1)) : 0);  // of all CTAs of the tile
+        auto boxes_of = [&](int n) { return (n + G8_XFEW - 1) / G8_XFEW; };  // of 32 rows
+        const int mine = rows_of(cr), other = PAIR ? rows_of(cr ^ 1) : 0;
+        const bool few = mine < G8_XR;
+        const int x_boxes = few ? boxes_of(mine) : 1;
+        const uint32_t bytes = WR * G8_BLOCK + (boxes_of(mine) + (PAIR ? boxes_of(other) : 0)) * (G8_XFEW * G8_BLOCK);  // of all CTAs
         const bool is_w = lane < S::W_BOXES, is_x = !is_w && lane - S::W_BOXES < x_boxes;
         const int b = is_w ? cr + lane : lane - S::W_BOXES;  // half of the weight rows, or box of token rows
         const int colbase = tile.cb * tile_cols;
@@ -640,6 +639,24 @@ static int dispatch8(const Gemm8Args& a, int tile, const void* x, const void* w,
                      : launch8<T, 256, true, SWIGLU>(a, x, w, s);
 }
 
+// Which tile a batch gets; the bits are the same. Measured on a B200 with the benchmark's layer (64 experts,
+// gate and up 2048 x 2048 with SwiGLU, down 2048 x 1024), us for the narrow / wide / pair tile:
+//   1 token     gate-up 10.3 / 13.0 / 14.4    down  6.9 /  8.2 /  9.6   (wide: fewer tiles than SMs)
+//   8 tokens            34.9 / 37.2 / 46.8         21.7 / 21.8 / 29.8
+//   64 tokens           48.8 / 51.1 / 66.1         29.1 / 27.7 / 39.3
+//   512 tokens          53.1 / 54.1 / 69.3         30.9 / 30.7 / 42.8   (64 rows per expert)
+//   1024 tokens         75.6 / 67.5 / 73.6         45.1 / 40.8 / 47.8
+//   4096 tokens          204 /  172 /  172          126 /  106 /  110
+//   8192 tokens          380 /  313 /  299                              (1024 rows per expert)
+// So: pairs from 768 rows per expert; the wide tile from 64, and for plain products below that too where
+// it gives every SM a tile; else the narrow one, which SwiGLU's shorter rows of results suit.
+static int choose_tile8(int rows, int experts, int n_out, bool swiglu, int sms) {
+  if (rows >= 768LL * experts) return 3;
+  if (rows > 64LL * experts) return 2;
+  const long long wide = (long long)(rows < experts ? rows : experts) * ((n_out + 255) / 256);
+  return !swiglu && wide >= sms ? 2 : 1;
+}
+
 }  // namespace sy
 
 extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const void* w, const float* w_scale,
@@ -672,7 +689,12 @@ extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const vo
   a.status = device_status_word();
   if (!a.status) return SY_ERR_CUDA;
   a.wait_ns = wait_limit_ns();
-  if (tile == 0) tile = rows <= 64LL * n_experts ? 1 : rows < 256LL * n_experts ? 2 : 3;
+  if (tile == 0) {
+    int sms = 0;
+    const int rc = device_sm_count(&sms);
+    if (rc != SY_OK) return rc;
+    tile = choose_tile8(rows, n_experts, n_out, swiglu != 0, sms);
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == SY_DTYPE_F16) return swiglu ? dispatch8<__half, true>(a, tile, x, w, s) : dispatch8<__half, false>(a, tile, x, w, s);
   return swiglu ? dispatch8<__nv_bfloat16, true>(a, tile, x, w, s) : dispatch8<__nv_bfloat16, false>(a, tile, x, w, s);
