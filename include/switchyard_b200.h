@@ -286,14 +286,17 @@ int sy_quantize_weight(const void* w, int n_mats, int n_rows, int k_dim, int dty
  * k_dim], w_scale [n_experts, blocks, ceil(k_dim / 128)]. swiglu: n_full = 2*n_out, gate rows then
  * up rows, blocks = 2 * ceil(n_out / 128) (each half's on its own), C = round16(silu(gate) * up).
  * Sums, scales and epilogue in float32, ONE rounding. scale 16-bit [rows] or NULL (not with swiglu).
+ * c_scale not NULL (swiglu only, n_out % 16 == 0): the result is rows for the next product: C e4m3
+ * [rows, n_out] and c_scale f32 [ceil(n_out / 128), rows], with m as above over a row's 128 columns
+ * c_scale = m / 448 and C = e4m3(v * (448 / m)) of the float32 values v; dtype is not looked at.
  * offsets int32 [n_experts + 1]; values outside [0, rows] are clamped, rows of no expert are set to
  * zero. A row's bits do not depend on the other rows of its expert or on the tile.
- * tile: 0 = chosen from the mean rows per expert; 1 = 128 rows x 128 weight rows, 2 = 128 x 256,
- * 3 = 256 x 256 over a pair of CTAs. k_dim % 16 == 0, n_out % 8 == 0, n_experts <= 256, x, w and C
+ * tile: 0 = chosen from the mean rows per expert; 1 = 128 rows x 128 weight rows (not with c_scale),
+ * 2 = 128 x 256, 3 = 256 x 256 over a pair of CTAs. k_dim % 16 == 0, n_out % 8 == 0, n_experts <= 256, x, w and C
  * 16-byte aligned. */
 int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const void* w, const float* w_scale, const int32_t* offsets,
-                        int n_experts, int rows, int n_out, int k_dim, int swiglu, const void* scale, void* C, int dtype,
-                        int tile, void* stream);
+                        int n_experts, int rows, int n_out, int k_dim, int swiglu, const void* scale, void* C,
+                        float* c_scale, int dtype, int tile, void* stream);
 
 /* ---- expert parallelism over device-driven transport ----------------------------------------
  * The entry points below have no single counterpart in the reference: together they replace

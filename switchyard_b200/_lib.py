@@ -60,7 +60,7 @@ SYMBOLS = {
                                  c_void_p]),
     "sy_quantize_weight": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "sy_grouped_gemm_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
-                                    c_void_p, c_void_p, c_int, c_int, c_void_p]),
+                                    c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "sy_grouped_segments": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                     c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "sy_ep_dispatch_scratch_bytes": (c_size_t, [c_int]),

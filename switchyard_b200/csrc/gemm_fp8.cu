@@ -4,6 +4,8 @@
 //   acc[r, n] = sum_b sx[b, r] * sw[e, n / 128, b] * sum_{k in block b} x[r, k] * w[e, n, k]
 //   C[r, n]   = round(acc[r, n] * scale[r])   or, with SwiGLU, round(silu(acc[r, gate n]) * acc[r, up n])
 //
+// or that SwiGLU result as e4m3 with scales for 128 columns, which is what the down projection reads.
+//
 // Float32 scales cannot ride in the tensor core, so the inner sums of each block of 128 (four
 // tcgen05.mma of k = 32) go to tensor memory on their own and eight warps multiply them by the
 // two scales and add them up in float32 registers while the next block is being multiplied:
@@ -20,6 +22,7 @@
 // TMA box (a box takes its thread about 130 clocks to issue, however small: six to eight boxes a
 // stage took twice as long as the multiplication).
 #include <cuda.h>
+#include <cuda_fp8.h>
 
 #include <atomic>
 #include <string.h>
@@ -72,6 +75,7 @@ struct Gemm8Args {
   const int* offsets;   // [experts + 1]
   const void* scale;    // [rows] or null
   void* C;              // [rows, Nout]
+  float* cscale;        // 8-bit results: [Nout blocks][rows]
   int experts, rows, Nout, K;
   int* status;
   unsigned long long wait_ns;
@@ -165,6 +169,11 @@ template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, 
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return reinterpret_cast<const uint32_t&>(v);
 }
+__device__ __forceinline__ uint64_t pair64(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
 __device__ __forceinline__ float2 both(uint64_t v) {
   float2 f;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
@@ -224,6 +233,8 @@ __device__ __forceinline__ float2 swiglu32(float2 g, float2 u) {
 template <typename T, int WR, bool PAIR, bool SWIGLU>
 __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(const __grid_constant__ Gemm8Args args) {
   using S = Shape8<WR, PAIR>;
+  constexpr bool OUT8 = std::is_same<T, __nv_fp8_e4m3>::value;
+  static_assert(!OUT8 || (SWIGLU && WR == 256), "a tile of SwiGLU columns is one block of 128");
   constexpr int STAGES = S::STAGES, BUFS = S::BUFS;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES];
@@ -234,6 +245,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
   __shared__ int s_begin[G8_MAX_E], s_end[G8_MAX_E];
   __shared__ int s_tile_start[G8_MAX_E + 1];
   __shared__ float s_scale[G8_SLOTS][G8_SLOT];
+  __shared__ float s_top[OUT8 ? 2 : 1][OUT8 ? 2 : 1][G8_XR];  // 8-bit results: largest magnitude of a row in either 64 columns
   __shared__ __align__(16) unsigned char s_out[S::PROMOTERS][32 * G8_OUT_PITCH];
 
   // (uniform to the compiler, so that the roles are too)
@@ -395,8 +407,11 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
     } else {
       // -------------------------------------------------------------- scales (and the rows of no expert)
       for (int r = (int)blockIdx.x, lo = s_begin[0], hi = s_end[E - 1]; r < lo + (args.rows - hi); r += (int)gridDim.x) {
-        uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(args.C) + (size_t)(r < lo ? r : hi + (r - lo)) * Nout);
-        for (int c = lane; c < Nout / 8; c += 32) row[c] = make_uint4(0u, 0u, 0u, 0u);
+        const size_t at = r < lo ? r : hi + (r - lo);
+        uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(args.C) + at * Nout);
+        for (int c = lane; c < Nout * (int)sizeof(T) / 16; c += 32) row[c] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (OUT8)
+          for (int b = lane; b < (Nout + G8_BLOCK - 1) / G8_BLOCK; b += 32) args.cscale[(size_t)b * args.rows + at] = 0.f;
       }
       // Every block's scales are copied asynchronously, G8_AHEAD blocks before their turn: the first
       // ones come from DRAM, behind the weights. (Loads into registers are no ring: waiting for an
@@ -456,7 +471,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
     const int q = warp & 3, g = (warp - G8_HELPERS) >> 2;  // quarter of the lanes; quarter of the columns: COLS of either half
     const int trow = cr * G8_XR + q * 32 + lane;
     const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + g * S::COLS;
-    int it = 0, cursor = 0;
+    int it = 0, cursor = 0, parity = 0;
     bool alive = true;
     Tile8 next;
     if (unit < total_tiles) next = locate_tile8<S::BM>(unit, cursor, E, s_tile_start, s_begin, s_end);
@@ -464,7 +479,8 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
       const Tile8 tile = next;
       const bool busy = cr * G8_XR + q * 32 < tile.nvalid;  // the warp has rows of this tile
       float row_scale = 1.f;
-      if (!SWIGLU && args.scale && trow < tile.nvalid) row_scale = Elem<T>::to_f(static_cast<const T*>(args.scale)[tile.row0 + trow]);
+      if constexpr (!SWIGLU)
+        if (args.scale && trow < tile.nvalid) row_scale = Elem<T>::to_f(static_cast<const T*>(args.scale)[tile.row0 + trow]);
       uint64_t acc[2][S::COLS / 2];
 #pragma unroll
       for (int j = 0; j < S::COLS / 2; ++j) acc[0][j] = acc[1][j] = 0;
@@ -514,12 +530,13 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
           next = locate_tile8<S::BM>(t + units, cursor, E, s_tile_start, s_begin, s_end);
       }
       alive = __all_sync(0xffffffffu, alive);
-      if (!alive || !busy) continue;
+      if (!busy || (!alive && !OUT8)) continue;  // (8-bit results: the warp of the same rows waits at a barrier below)
       const int rows = tile.nvalid - (cr * G8_XR + q * 32), col = tile.cb * tile_cols + g * S::COLS;
       T* to = static_cast<T*>(args.C) + (size_t)(tile.row0 + cr * G8_XR + q * 32) * Nout + col;
-      // Thirty-two columns from col + c on, a row per lane, to memory by way of shared memory: a store
-      // then covers eight rows of 64 bytes, where a lane's own row would make it touch 32 lines.
-      auto store32 = [&](int c, const uint32_t (&o)[16]) {
+      // 64 bytes of results per lane, its row's from column col + c on, to memory by way of shared memory:
+      // a store then covers eight rows of 64 bytes, where a lane's own row would make it touch 32 lines.
+      auto store64 = [&](int c, const uint32_t (&o)[16]) {
+        constexpr int PART = 16 / sizeof(T);
         unsigned char* mine = s_out[warp - G8_HELPERS] + lane * G8_OUT_PITCH;
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(mine + i * 16) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -529,11 +546,46 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         for (int i = 0; i < 4; ++i) {
           const int r = i * 8 + (lane >> 2);
           const uint4 v = *reinterpret_cast<const uint4*>(s_out[warp - G8_HELPERS] + r * G8_OUT_PITCH + part * 16);
-          if (r < rows && col + c + part * 8 < Nout) *reinterpret_cast<uint4*>(to + (size_t)r * Nout + c + part * 8) = v;
+          if (r < rows && col + c + part * PART < Nout)
+            *reinterpret_cast<uint4*>(to + (size_t)r * Nout + c + part * PART) = v;
         }
         __syncwarp();
       };
-      if constexpr (SWIGLU) {
+      if constexpr (OUT8) {
+        // The row's 128 columns are a block: its largest magnitude over this warp's 64 and, through shared
+        // memory, over those of the warp that has the other half. A value is rounded from its product
+        // with 448 / m; it comes out of float32 sums, so there are no midpoints to keep.
+        float top = 0.f;
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < S::COLS / 2; ++j) {
+          const float2 v = swiglu32(both(acc[0][j]), both(acc[1][j]));
+          acc[0][j] = pair64(v);
+          if (col + 2 * j < Nout) {  // Nout is even
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+            nan |= v.x != v.x || v.y != v.y;
+          }
+        }
+        if (nan) top = __int_as_float(0x7fffffff);
+        float(*half)[G8_XR] = s_top[parity];
+        half[g][q * 32 + lane] = top;
+        named_barrier_sync(1 + q, 64);
+        const float other = half[g ^ 1][q * 32 + lane];
+        top = top != top || other != other ? __int_as_float(0x7fffffff) : fmaxf(fmaxf(top, other), 0x1p-96f);
+        parity ^= 1;
+        if (!alive) continue;
+        const float inv = 448.f / top;
+        uint32_t o[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float2 a = both(acc[0][2 * j]), b = both(acc[0][2 * j + 1]);
+          o[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a.x * inv, a.y * inv), __NV_SATFINITE, __NV_E4M3) |
+                 ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(b.x * inv, b.y * inv), __NV_SATFINITE, __NV_E4M3) << 16);
+        }
+        store64(0, o);
+        if (g == 0 && lane < rows)
+          args.cscale[(size_t)(col / G8_BLOCK) * args.rows + tile.row0 + trow] = top / 448.f;
+      } else if constexpr (SWIGLU) {
 #pragma unroll
         for (int c = 0; c < S::COLS; c += 32) {
           uint32_t o[16];
@@ -542,7 +594,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
             const float2 v = swiglu32(both(acc[0][c / 2 + j]), both(acc[1][c / 2 + j]));
             o[j] = pack16<T>(v.x, v.y);
           }
-          store32(c, o);
+          store64(c, o);
         }
       } else {
 #pragma unroll
@@ -553,7 +605,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
             const float2 v = both(acc[c / S::COLS][c % S::COLS / 2 + j]);
             o[j] = pack16<T>(v.x * row_scale, v.y * row_scale);
           }
-          store32(c < S::COLS ? c : WR / 2 + c - S::COLS, o);
+          store64(c < S::COLS ? c : WR / 2 + c - S::COLS, o);
         }
       }
     }
@@ -634,9 +686,9 @@ static int launch8(Gemm8Args a, const void* x, const void* w, cudaStream_t strea
 
 template <typename T, bool SWIGLU>
 static int dispatch8(const Gemm8Args& a, int tile, const void* x, const void* w, cudaStream_t s) {
-  return tile == 1   ? launch8<T, 128, false, SWIGLU>(a, x, w, s)
-         : tile == 2 ? launch8<T, 256, false, SWIGLU>(a, x, w, s)
-                     : launch8<T, 256, true, SWIGLU>(a, x, w, s);
+  if constexpr (!std::is_same<T, __nv_fp8_e4m3>::value)
+    if (tile == 1) return launch8<T, 128, false, SWIGLU>(a, x, w, s);
+  return tile == 2 ? launch8<T, 256, false, SWIGLU>(a, x, w, s) : launch8<T, 256, true, SWIGLU>(a, x, w, s);
 }
 
 // Which tile a batch gets; the bits are the same. Measured on a B200 with the benchmark's layer (64 experts,
@@ -661,14 +713,16 @@ static int choose_tile8(int rows, int experts, int n_out, bool swiglu, int sms) 
 
 extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const void* w, const float* w_scale,
                                    const int32_t* offsets, int n_experts, int rows, int n_out, int k_dim, int swiglu,
-                                   const void* scale, void* C, int dtype, int tile, void* stream) {
+                                   const void* scale, void* C, float* c_scale, int dtype, int tile, void* stream) {
   using namespace sy;
   SY_REQUIRE(rows >= 0 && n_experts >= 1 && n_experts <= G8_MAX_E, "grouped_gemm_fp8: 1..%d experts (got %d)", G8_MAX_E,
              n_experts);
   SY_REQUIRE(k_dim > 0 && k_dim % 16 == 0, "grouped_gemm_fp8: k_dim must be a multiple of 16 (got %d)", k_dim);
   SY_REQUIRE(n_out > 0 && n_out % 8 == 0, "grouped_gemm_fp8: n_out must be a multiple of 8 (got %d)", n_out);
   SY_REQUIRE(!(swiglu && scale), "grouped_gemm_fp8: swiglu and scale are separate epilogues");
-  SY_REQUIRE(dtype == SY_DTYPE_F16 || dtype == SY_DTYPE_BF16, "grouped_gemm_fp8: dtype must be f16 or bf16");
+  SY_REQUIRE(c_scale || dtype == SY_DTYPE_F16 || dtype == SY_DTYPE_BF16, "grouped_gemm_fp8: dtype must be f16 or bf16");
+  SY_REQUIRE(!c_scale || (swiglu && n_out % 16 == 0 && tile != 1),
+             "grouped_gemm_fp8: 8-bit results are SwiGLU's, of a multiple of 16 columns, from the wide tiles");
   SY_REQUIRE(tile >= 0 && tile <= 3, "grouped_gemm_fp8: tile 0..3 (got %d)", tile);
   SY_REQUIRE((int64_t)n_experts * 2 * n_out <= 0x7fffffff, "grouped_gemm_fp8: more than 2^31 weight rows");
   if (rows == 0) return SY_OK;
@@ -682,6 +736,7 @@ extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const vo
   a.offsets = offsets;
   a.scale = scale;
   a.C = C;
+  a.cscale = c_scale;
   a.experts = n_experts;
   a.rows = rows;
   a.Nout = n_out;
@@ -694,8 +749,10 @@ extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const vo
     const int rc = device_sm_count(&sms);
     if (rc != SY_OK) return rc;
     tile = choose_tile8(rows, n_experts, n_out, swiglu != 0, sms);
+    if (c_scale && tile == 1) tile = 2;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c_scale) return dispatch8<__nv_fp8_e4m3, true>(a, tile, x, w, s);
   if (dtype == SY_DTYPE_F16) return swiglu ? dispatch8<__half, true>(a, tile, x, w, s) : dispatch8<__half, false>(a, tile, x, w, s);
   return swiglu ? dispatch8<__nv_bfloat16, true>(a, tile, x, w, s) : dispatch8<__nv_bfloat16, false>(a, tile, x, w, s);
 }

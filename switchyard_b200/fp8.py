@@ -77,19 +77,35 @@ def grouped_gemm(x, w, offsets, swiglu=False, scale=None, dtype=torch.bfloat16):
     """Every expert's rows times its weights: x Rows8 in expert order, w Weight8, offsets int32 [E+1].
     C [rows, N] = x w^T; with scale [rows] (dtype) every row times its own; with swiglu (w quantised
     in two halves) C [rows, N/2] = silu(x gate^T) * (x up^T). Float32 up to the one rounding to `dtype`
-    (bf16 or fp16). Rows of no expert are zero. A row's bits depend on nothing but the row and its
-    expert's weights."""
+    (bf16 or fp16). dtype float8_e4m3fn, with swiglu: the result as Rows8 for the next product, quantised
+    where it is computed (scale = m / 448 and q = e4m3(v * (448 / m)) of the float32 values). Rows of no
+    expert are zero. A row's bits depend on nothing but the row and its expert's weights."""
     _no_grad("grouped_gemm", scale)
-    return _rows._ext().grouped_gemm_fp8(x.q, x.scale, w.q, w.scale, offsets, swiglu, scale, dtype)
+    out = _rows._ext().grouped_gemm_fp8(x.q, x.scale, w.q, w.scale, offsets, swiglu, scale, dtype)
+    return Rows8(*out) if dtype is torch.float8_e4m3fn else out
+
+
+# "auto" is "gemv" up to this many rows per expert on average, where the product's narrow tile applies. The
+# benchmark's layer, graph replays, us for gemv / gemm: 8 tokens 87.5 / 86.1, 64 107 / 109, 256 115 / 117,
+# 512 (64 rows per expert) 122 / 119, 1024 155 / 150, 4096 413 / 381, 8192 732 / 685.
+AUTO_GEMV_MAX_MEAN_ROWS = 64
 
 
 def sorted_experts(h, plan, wsorted, gate_up, down, mode="auto"):
     """The expert FFN on 8-bit weights for a sorted batch: rows quantised into expert order, gate/up
-    product with SwiGLU, its result quantised, down product times the router weights wsorted.
-    Returns y [N*k, H] in h's dtype, for combine. `mode` is checked and otherwise without effect."""
+    product with SwiGLU, its result in 8 bits, down product times the router weights wsorted. Mode "gemv"
+    (decode): the SwiGLU result is rounded to h's dtype and quantised by a launch of its own; "gemm" (and
+    "cublas"): quantised from float32 where it is computed. The two are separate contracts, within each a
+    row's bits do not depend on the batch; "auto" chooses from the mean rows per expert.
+    Returns y [N*k, H] in h's dtype, for combine."""
     if mode not in ("auto", "gemv", "gemm", "cublas"):
         raise RuntimeError(f"sorted_experts: unknown mode {mode!r}")
     if not (isinstance(gate_up, Weight8) and isinstance(down, Weight8)):
         raise RuntimeError("sorted_experts: gate_up and down must both be 8-bit (fp8.Weight8) or both 16-bit")
-    act = grouped_gemm(quantize_rows(h, plan), gate_up, plan.offsets, swiglu=True, dtype=h.dtype)
-    return grouped_gemm(quantize_rows(act), down, plan.offsets, scale=wsorted, dtype=h.dtype)
+    few = plan.pos_of.numel() <= AUTO_GEMV_MAX_MEAN_ROWS * gate_up.q.shape[0] if mode == "auto" else mode == "gemv"
+    x = quantize_rows(h, plan)
+    if few:
+        act = quantize_rows(grouped_gemm(x, gate_up, plan.offsets, swiglu=True, dtype=h.dtype))
+    else:
+        act = grouped_gemm(x, gate_up, plan.offsets, swiglu=True, dtype=torch.float8_e4m3fn)
+    return grouped_gemm(act, down, plan.offsets, scale=wsorted, dtype=h.dtype)

@@ -17,7 +17,7 @@ Differences a caller can observe:
     the largest expert's row count, so the layer never synchronises;
   * `experts`, `moe_layer` and `GraphedLayer` also take 8-bit expert weights (`fp8.Weight8` for both
     gate_up and down): the rows are then quantised on their way into expert order and both
-    products run in e4m3, whatever `mode` says (the tile follows the batch, the bits do not);
+    products run in e4m3 (`fp8.sorted_experts` says what `mode` chooses there);
   * `route_fused` computes the router logits inside the routing launch instead of calling the
     library GEMM. It is not what `moe_layer` uses unless SWITCHYARD_FUSED_ROUTER=1 (or
     `route_and_sort(..., fused=True)`): measured on a B200 the library GEMM followed by the
@@ -421,7 +421,8 @@ class Ext:
         return q, scale
 
     def grouped_gemm_fp8(self, x, x_scale, w, w_scale, offsets, swiglu, scale, dtype, tile=0):
-        """The experts' product of 8-bit rows and weights (sy_grouped_gemm_fp8): C [rows, n_out]."""
+        """The experts' product of 8-bit rows and weights (sy_grouped_gemm_fp8): C [rows, n_out] in dtype;
+        with dtype float8_e4m3fn (swiglu only) C and its scales [ceil(n_out/128), rows]."""
         name = "grouped_gemm_fp8"
         dev = _on_device(x, name)
         for t, what, dt, dims in ((x, "x", torch.float8_e4m3fn, 2), (x_scale, "x_scale", torch.float32, 2),
@@ -439,18 +440,20 @@ class Ext:
         if w_scale.shape != (E, parts * ((n_out + 127) // 128), kb):
             raise RuntimeError(f"{name}: w_scale must be [{E}, {parts * ((n_out + 127) // 128)}, {kb}], got "
                                f"{list(w_scale.shape)}" + (" (quantise gate and up as two halves)" if swiglu else ""))
-        if dtype is not torch.float16 and dtype is not torch.bfloat16:
-            raise RuntimeError(f"{name}: the result is fp16 or bf16, not {dtype}")
+        out8 = dtype is torch.float8_e4m3fn
+        if dtype is not torch.float16 and dtype is not torch.bfloat16 and not (out8 and swiglu):
+            raise RuntimeError(f"{name}: the result is fp16 or bf16, or e4m3 with swiglu, not {dtype}")
         if scale is not None and (scale.dtype is not dtype or scale.shape != (rows,) or _on_device(scale, name, "scale") != dev):
             raise RuntimeError(f"{name}: scale must be [{rows}] in the result's dtype, on x's device")
         C = torch.empty((rows, n_out), dtype=dtype, device=x.device)
+        c_scale = torch.empty(((n_out + 127) // 128, rows), dtype=torch.float32, device=x.device) if out8 else None
         code = _lib.SY_DTYPE_F16 if dtype is torch.float16 else _lib.SY_DTYPE_BF16
         with _Device(dev) as stream:
             rc = self.lib.sy_grouped_gemm_fp8(x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
                                               offsets.data_ptr(), E, rows, n_out, K, 1 if swiglu else 0, _ptr(scale),
-                                              C.data_ptr(), code, int(tile), stream)
+                                              C.data_ptr(), _ptr(c_scale), code, int(tile), stream)
         _lib.check(rc, name)
-        return C
+        return (C, c_scale) if out8 else C
 
     def gather_rows(self, src, index, dst):
         _check(src, "src"), _check(index, "index"), _check(dst, "dst")

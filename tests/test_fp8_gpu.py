@@ -144,6 +144,43 @@ def test_grouped_gemm(Q, counts, K, N, dtype, kind):
         assert torch.equal(again.isnan(), got.isnan()) and torch.equal(again[~nan], got[~nan]), tile
 
 
+@pytest.mark.parametrize("counts,K,N", [(c, k, n) for c, k, n in SHAPES if n % 16 == 0] + [([5, 0, 140], 128, 400), ([300], 256, 1040)])
+def test_swiglu_straight_to_8_bits(Q, counts, K, N):
+    """The SwiGLU result as Rows8. With v the exact value, d the bound of its float32 one and M the block's
+    exact largest magnitude: the scale is within d's maximum (and three roundings) of M / 448, and
+    q * scale is v up to d, half a step of e4m3 (2^-4 of the value, or half its least subnormal, 2^-10
+    scales) and the roundings of 448 / m, of the product and of the scale."""
+    from switchyard_b200 import kernels
+    offsets, xq, xs, wq, ws = operands(counts, K, N, True, 2 * K + N)
+    acc, mag = product64(xq, xs, wq, ws, offsets, True, None)
+    ref, bound = swiglu_bound(acc, mag, K, N, F32)
+    dev = [t.to(DEV) for t in (xq, xs, wq, ws, offsets)]
+    got = Q.grouped_gemm(Q.Rows8(*dev[:2]), Q.Weight8(*dev[2:4]), dev[4], swiglu=True, dtype=torch.float8_e4m3fn)
+    M, blocks = xq.shape[0], -(-N // 128)
+    assert got.q.dtype == torch.float8_e4m3fn and got.q.shape == (M, N) and got.scale.shape == (blocks, M)
+    q, scale = got.q.cpu().double(), got.scale.cpu().double()
+    for b in range(blocks):
+        cols = slice(b * 128, min(N, b * 128 + 128))
+        v, d, s = ref[:, cols], bound[:, cols], scale[b]
+        bad = v.isnan().any(1)  # a NaN makes its row's block NaN
+        assert torch.equal(s.isnan(), bad) and q[:, cols][bad].isnan().all()
+        v, d, s, c = v[~bad], d[~bad], s[~bad], q[:, cols][~bad]
+        m = v.abs().amax(1)
+        assert ((s * 448 - m.clamp(min=2.0 ** -96)).abs() <= d.amax(1) + 2.0 ** -22 * m).all()
+        far = d + (v.abs() + d) * (2.0 ** -4 + 2.0 ** -21) + 2.0 ** -10 * s[:, None]
+        assert ((c * s[:, None] - v).abs() <= far).all()
+    for tile in (2, 3):
+        again = kernels.ext().grouped_gemm_fp8(*dev, True, None, torch.float8_e4m3fn, tile)
+        assert torch.equal(again[0].view(torch.uint8), got.q.view(torch.uint8))
+        assert torch.equal(again[1].view(torch.int32), got.scale.view(torch.int32))
+    # rows of no expert: zero values and scales
+    short = dev[4].clone()
+    short[-1] = max(int(short[-2]), int(short[-1]) - 1)
+    less = Q.grouped_gemm(Q.Rows8(*dev[:2]), Q.Weight8(*dev[2:4]), short, swiglu=True, dtype=torch.float8_e4m3fn)
+    assert (less.q[int(short[-1]):].float() == 0).all() and (less.scale[:, int(short[-1]):] == 0).all()
+    assert torch.equal(less.q[:int(short[-1])].view(torch.uint8), got.q[:int(short[-1])].view(torch.uint8))
+
+
 def test_a_rows_bits_do_not_depend_on_its_expert_s_other_rows(Q):
     from switchyard_b200 import kernels
     offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([200], 384, 160, False, 3))
@@ -196,9 +233,10 @@ def layer(N, E, k, H, I, dtype, seed=0):
 @pytest.mark.parametrize("N,E,k,H,I,dtype", [(1, 64, 8, 256, 128, BF), (7, 8, 2, 128, 48, HF), (64, 64, 8, 256, 128, HF),
                                              (333, 64, 8, 256, 144, BF), (2100, 8, 4, 256, 128, BF), (0, 8, 2, 128, 64, BF)])
 def test_the_layer_on_8_bit_experts(Q, N, E, k, H, I, dtype):
-    """moe_layer with Weight8 experts: route, sort, quantise into expert order, product with SwiGLU,
-    quantise, product with router weights, combine: the bits of the operators called one by one,
-    in every mode, with a residual and through GraphedLayer; and near the 16-bit layer."""
+    """moe_layer with Weight8 experts: route, sort, quantise into expert order, product with SwiGLU and
+    its result to 8 bits ("gemv": by a launch of its own, "gemm": where it is computed), product
+    with router weights, combine: the bits of the operators called one by one, with a residual and
+    through GraphedLayer too; and near the 16-bit layer."""
     from switchyard_b200 import kernels, rows
     h, router, gate_up, down = layer(N, E, k, H, I, dtype)
     gu8, dn8 = Q.quantize_weight(gate_up, halves=2), Q.quantize_weight(down)
@@ -208,11 +246,13 @@ def test_the_layer_on_8_bit_experts(Q, N, E, k, H, I, dtype):
         return
     idx, w, counts, offsets, token, wsorted, pos_of = kernels.route_and_sort(h, router, k, False)
     plan = rows.SortPlan(counts, offsets, token, pos_of.view(N, k))
-    act = Q.grouped_gemm(Q.quantize_rows(h, plan), gu8, offsets, swiglu=True, dtype=dtype)
-    y = Q.grouped_gemm(Q.quantize_rows(act), dn8, offsets, scale=wsorted, dtype=dtype)
-    assert torch.equal(out, kernels.ext().combine(y, pos_of, idx, N))
-    for mode in ("gemv", "gemm"):
-        assert torch.equal(kernels.moe_layer(h, router, gu8, dn8, k, False, mode), out)
+    x8 = Q.quantize_rows(h, plan)
+    acts = {"gemv": Q.quantize_rows(Q.grouped_gemm(x8, gu8, offsets, swiglu=True, dtype=dtype)),
+            "gemm": Q.grouped_gemm(x8, gu8, offsets, swiglu=True, dtype=torch.float8_e4m3fn)}
+    for mode, act in acts.items():
+        y = Q.grouped_gemm(act, dn8, offsets, scale=wsorted, dtype=dtype)
+        assert torch.equal(kernels.moe_layer(h, router, gu8, dn8, k, False, mode), kernels.ext().combine(y, pos_of, idx, N))
+    assert torch.equal(out, kernels.moe_layer(h, router, gu8, dn8, k, False, "gemv" if N * k <= 64 * E else "gemm"))
     assert torch.equal(kernels.experts(h, idx, w, gu8, dn8), out)
     x = torch.randn_like(h)
     assert torch.equal(kernels.moe_layer(h, router, gu8, dn8, k, False, residual=x), x + out)
@@ -258,7 +298,7 @@ def test_refusals(Q):
     bad = [dict(x=x._replace(scale=xs.t())), dict(x=x._replace(q=xq.float())), dict(w=w._replace(scale=ws[:1])),
            dict(w=w._replace(q=wq.cpu())), dict(offsets=offsets[:2]), dict(offsets=offsets.long()), dict(dtype=F32),
            dict(scale=torch.ones(8, device=DEV)), dict(scale=torch.ones(7, device=DEV, dtype=BF)),
-           dict(swiglu=True, scale=torch.ones(8, device=DEV, dtype=BF))]
+           dict(swiglu=True, scale=torch.ones(8, device=DEV, dtype=BF)), dict(dtype=torch.float8_e4m3fn)]
     for change in bad:
         with pytest.raises(RuntimeError):
             Q.grouped_gemm(**{**dict(x=x, w=w, offsets=offsets), **change})

@@ -54,14 +54,17 @@ def test_quantisers_and_the_product_refuse(lib):
     refused(lib, lib.sy_quantize_weight(P, 1, 0, 64, 1, P, P, None), b"rows")
     refused(lib, lib.sy_quantize_weight(P, 1 << 20, 8, 64, 1, P, P, None), b"matrices")
     refused(lib, lib.sy_quantize_weight(P, 1, 8, 40, 1, P, P, None), b"multiple of 16")
-    args = lambda E=8, rows=4, n=64, k=128, sw=0, scale=None, dt=1, tile=0, x=P: (x, P, P, P, P, E, rows, n, k, sw, scale, P, dt,
-                                                                               tile, None)
+    args = lambda E=8, rows=4, n=64, k=128, sw=0, scale=None, dt=1, tile=0, x=P, cs=None: (x, P, P, P, P, E, rows, n, k, sw, scale, P,
+                                                                                        cs, dt, tile, None)
     refused(lib, lib.sy_grouped_gemm_fp8(*args(E=257)), b"experts")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(k=120)), b"multiple of 16")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(n=60)), b"multiple of 8")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(sw=1, scale=P)), b"separate")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(dt=2)), b"dtype")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(tile=4)), b"tile")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(cs=P)), b"SwiGLU")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(cs=P, sw=1, n=72)), b"multiple of 16")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(cs=P, sw=1, tile=1)), b"wide")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(x=None)), b"null")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(x=ctypes.c_void_p(8))), b"aligned")
     assert lib.sy_grouped_gemm_fp8(*args(rows=0, x=None)) == 0
