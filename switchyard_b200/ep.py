@@ -42,6 +42,8 @@ from concurrent.futures import ThreadPoolExecutor
 
 import torch
 
+from . import fp8
+
 DEFAULT_MAX_TOKENS = 4096
 
 
@@ -429,6 +431,7 @@ class ExpertParallel:
         """hs[r]: [N_r, H] hidden states of rank r's tokens; routers[r]: the layer's router (on
         every rank); gate_ups[r], downs[r]: rank r's experts. Returns the MoE output for every
         rank's tokens. All ranks driven from this thread (switchyard/ep.py:274-285)."""
+        fp8.refuse("layer", *gate_ups, *downs)
         if self.windows:
             self.reserve(max(h.shape[0] for h in hs))
         state = self.new_state()
@@ -444,6 +447,7 @@ class ExpertParallel:
         """Rank r's part of one layer, from rank r's thread (switchyard/ep.py:289-296). Ranks whose
         phases are ordered on the host meet at the barrier between phases; ranks on distinct GPUs
         over windows do not meet at all: their kernels wait for each other's flags."""
+        fp8.refuse("layer_rank", gate_up, down)
         meet = self.barrier.wait if self.host_ordered else (lambda: None)
         self.phase_send(sh, r, h, router)
         meet()

@@ -31,7 +31,7 @@ import ctypes
 import torch
 import torch.distributed as dist
 
-from . import _lib, kernels
+from . import _lib, fp8, kernels
 from .ep_window import Channel, window_layout  # noqa: F401  (window_layout is part of this module's API)
 
 
@@ -135,6 +135,7 @@ class DistributedExpertParallel:
         Returns [N,H]; with residual [N,H] (contiguous, h's dtype) residual + layer(h), added in the
         combine launch with the bits of the separate 16-bit addition. Collective: every rank must
         call it once per layer, in the same order."""
+        fp8.refuse("layer", gate_up, down)
         N = h.shape[0]
         if residual is not None and (residual.shape != h.shape or residual.dtype != h.dtype
                                      or not residual.is_contiguous()):

@@ -50,6 +50,12 @@ class Weight8(NamedTuple):
         return (self.q.float() * s.reshape(E, N, K)).to(dtype)
 
 
+def refuse(name, *weights):
+    """Raises where a path that has 16-bit experts only is given 8-bit ones."""
+    if any(isinstance(w, Weight8) for w in weights):
+        raise RuntimeError(f"{name}: 8-bit experts (fp8.Weight8) are for one GPU; pass the 16-bit stacks")
+
+
 def _no_grad(name, t):
     if t is not None and t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")

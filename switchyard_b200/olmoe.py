@@ -104,6 +104,16 @@ def from_hf_state_dict(sd, c, dtype=torch.float32, device="cpu"):
     return w
 
 
+def quantize_experts(weights):
+    """The same weights with every layer's expert stacks in 8 bits (fp8.Weight8), for hooks that call
+    `kernels.moe_layer`; everything else is shared. Layer by layer: drop the 16-bit ones to free
+    their memory."""
+    from . import fp8
+    layers = [{**L, "gate_up": fp8.quantize_weight(L["gate_up"], halves=2), "down": fp8.quantize_weight(L["down"])}
+              for L in weights["layers"]]
+    return {**weights, "layers": layers}
+
+
 def scaled_norm(x, weight, eps):
     """RMS normalisation computed in float32, result in x's dtype, times the learned scale."""
     return weight * F.rms_norm(x.float(), (x.shape[-1],), eps=eps).to(x.dtype)

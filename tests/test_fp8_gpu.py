@@ -267,6 +267,27 @@ def test_the_layer_on_8_bit_experts(Q, N, E, k, H, I, dtype):
     assert (out.double() - ref).norm() <= 0.25 * ref.norm()
 
 
+def test_the_decoder_on_8_bit_experts(Q):
+    """olmoe.quantize_experts: the model's own hook on 8-bit experts. A replayed decode step gives the eager
+    one's bits, tokens are generated, and the logits stay near the 16-bit model's: per layer the MoE
+    output moves by at most 4 * 2^-4 of itself (four operands rounded to e4m3), and what a layer adds
+    is a part of the residual stream, so three layers move the normalised stream by less than 0.75."""
+    from switchyard_b200 import kernels, olmoe
+    c = olmoe.Config(vocab=211, hidden=256, intermediate=128, layers=3, heads=4, kv_heads=2, head_dim=64, experts=16, top_k=4,
+                     max_positions=128)
+    w = olmoe.random_weights(c, DEV, HF, seed=3, std=0.06)
+    def decoder(w):
+        hook = lambda i, h: kernels.moe_layer(h, w["layers"][i]["router"], w["layers"][i]["gate_up"], w["layers"][i]["down"],
+                                              c.top_k, c.norm_topk_prob, "gemv")
+        return olmoe.Decoder(c, w, hook)
+    d16, d8 = decoder(w), decoder(olmoe.quantize_experts(w))
+    toks = torch.randint(3, c.vocab, (3, 11), generator=torch.Generator().manual_seed(8)).to(DEV)
+    a, b = d16.forward(toks).double(), d8.forward(toks).double()
+    assert (a - b).norm() <= 0.75 * a.norm()
+    prompts = [toks[0].tolist(), toks[1, :6].tolist()]
+    assert d8.generate(prompts, 8, graph=True) == d8.generate(prompts, 8, graph=False)
+
+
 def test_streams_and_graphs(Q):
     """The same call on two streams at once and replayed from a graph, on new inputs."""
     offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([20, 0, 300], 256, 256, True, 9))

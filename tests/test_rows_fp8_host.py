@@ -116,3 +116,14 @@ def test_dequantize_is_the_layout(lib):
     w8 = fp8.Weight8(torch.stack([a for a, _ in parts]).view(2, 272, 144).float().to(torch.float8_e4m3fn),
                      torch.stack([b for _, b in parts]).view(2, 4, 2))
     assert ((w8.dequantize(halves=2) - w).abs() <= w.abs() * (2.0 ** -4 + 2.0 ** -22) + 2.0 ** -10 * 6 / 448).all()
+
+
+def test_expert_parallelism_refuses_8_bit_experts(lib):
+    from switchyard_b200 import fp8
+    from switchyard_b200.ep import ExpertParallel
+    w8 = fp8.Weight8(torch.zeros(2, 64, 64).to(torch.float8_e4m3fn), torch.zeros(2, 1, 1))
+    ep = ExpertParallel(["cpu", "cpu"], 4, 2, False, ops=object())
+    with pytest.raises(RuntimeError, match="one GPU"):
+        ep.layer([torch.zeros(1, 64)] * 2, [torch.zeros(4, 64)] * 2, [w8, w8], [w8, w8])
+    with pytest.raises(RuntimeError, match="one GPU"):
+        ep.layer_rank(None, 0, torch.zeros(1, 64), torch.zeros(4, 64), w8, torch.zeros(2, 64, 32))
