@@ -7,20 +7,25 @@
 // or that SwiGLU result as e4m3 with scales for 128 columns, which is what the down projection reads.
 //
 // Float32 scales cannot ride in the tensor core, so the inner sums of each block of 128 (four
-// tcgen05.mma of k = 32) go to tensor memory on their own and eight warps multiply them by the
-// two scales and add them up in float32 registers while the next block is being multiplied:
-// tensor memory holds two such partial products of 256 columns, or four of 128. A thread owns a row of the tile and a half of its
-// columns. Both factors of a step are the same for all of a thread's columns of one weight block,
-// so the promotion costs one packed multiply-add per two values.
+// tcgen05.mma of k = 32) go to tensor memory on their own, and eight warps multiply them by the two
+// scales and add them up in float32 registers (the promotion) while the next block is being
+// multiplied: tensor memory holds two such partial products of 256 columns, or four of 128. A
+// thread owns a row of the tile and a quarter of its columns. Both scales are the same for all of a
+// thread's columns of one weight block, so a value costs half a packed multiply-add.
 //
 // Warps: 0 TMA producer, 1-2 MMA issuers, 3 scales, 4-11 promotion and epilogue.
 // Tiles as in gemm.cu: numbered on the device from `offsets`, expert-major, dealt round-robin to
 // a persistent grid. Token rows are the MMA's M operand (128, or 256 over a pair of CTAs), weight
-// rows its N operand, in two halves of WR / 2: consecutive rows, or with SwiGLU the gate rows and the
-// up rows of the same columns. A thread takes the same quarter of the columns out of either half:
-// it finds a gate value and its up value in its own registers, and each half of the tile is one
-// TMA box (a box takes its thread about 130 clocks to issue, however small: six to eight boxes a
-// stage took twice as long as the multiplication).
+// rows its N operand, in two halves of WR / 2 (a TMA box each): consecutive rows, or with SwiGLU the
+// gate rows and the up rows of the same columns. A thread takes the same quarter of the columns out
+// of either half, so that it finds a gate value and its up value in its own registers.
+//
+// What bounds it. Few rows per expert: the weights' way from HBM (64 tokens, 268 MB of gate and up: 48 us,
+// 5.6 TB/s). Many rows: the chain of one partial product, MMA - barrier - promotion - barrier - MMA,
+// against two buffers (950 clocks a block of 256 columns and two CTAs, where the MMAs alone take 512);
+// and, run for seconds, the GPU's power: 8192 tokens take 299 us in a burst at 1.65 GHz, 356 us at
+// 1.44 GHz and 990 W, of which the promotion's multiply-adds are 67 us. (The library's 8-bit product
+// of the same size, one scale per matrix, no experts, no SwiGLU, takes 246 us at the same power.)
 #include <cuda.h>
 #include <cuda_fp8.h>
 
@@ -365,10 +370,9 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full_bar[j % STAGES], (j / STAGES) & 1, 10000000ull);
     } else if (warp <= 2) {
       // -------------------------------------------------------------- MMA issuers (PAIR: the leader's, for both CTAs)
-      // Two warps take the k blocks in turn. A wait costs its warp 100 to 250
-      // clocks even when there is nothing to wait for; with one warp for all blocks those came
-      // one after another, 750 clocks a block.
-      // The whole warp walks the blocks (so that descriptors and loop counters stay in uniform
+      // Two warps take the k blocks in turn: a wait costs its warp 100 to 250 clocks even when there is
+      // nothing to wait for, and with one warp those came one after another, 750 clocks a block of 128
+      // columns instead of 560. The whole warp walks the blocks (so that descriptors and loop counters stay in uniform
       // registers), one elected lane issues.
       if (cr == 0) {
         const uint32_t ring_lo = umma_desc_lo(smem_u32(stages));
@@ -409,7 +413,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
       for (int r = (int)blockIdx.x, lo = s_begin[0], hi = s_end[E - 1]; r < lo + (args.rows - hi); r += (int)gridDim.x) {
         const size_t at = r < lo ? r : hi + (r - lo);
         uint4* row = reinterpret_cast<uint4*>(static_cast<T*>(args.C) + at * Nout);
-        for (int c = lane; c < Nout * (int)sizeof(T) / 16; c += 32) row[c] = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = lane; c < Nout / (16 / (int)sizeof(T)); c += 32) row[c] = make_uint4(0u, 0u, 0u, 0u);
         if constexpr (OUT8)
           for (int b = lane; b < (Nout + G8_BLOCK - 1) / G8_BLOCK; b += 32) args.cscale[(size_t)b * args.rows + at] = 0.f;
       }
@@ -724,7 +728,7 @@ extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const vo
   SY_REQUIRE(!c_scale || (swiglu && n_out % 16 == 0 && tile != 1),
              "grouped_gemm_fp8: 8-bit results are SwiGLU's, of a multiple of 16 columns, from the wide tiles");
   SY_REQUIRE(tile >= 0 && tile <= 3, "grouped_gemm_fp8: tile 0..3 (got %d)", tile);
-  SY_REQUIRE((int64_t)n_experts * 2 * n_out <= 0x7fffffff, "grouped_gemm_fp8: more than 2^31 weight rows");
+  SY_REQUIRE((int64_t)n_experts * 2 * n_out <= 0x7fffff00, "grouped_gemm_fp8: more than 2^31 weight rows");
   if (rows == 0) return SY_OK;
   SY_REQUIRE(x && x_scale && w && w_scale && offsets && C, "grouped_gemm_fp8: null pointer");
   SY_REQUIRE((uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && (uintptr_t)C % 16 == 0,

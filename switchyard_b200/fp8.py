@@ -8,7 +8,8 @@ multiplies. Beyond the reference, which has 16-bit experts only.
     out = kernels.moe_layer(h, router, gate_up8, down8, top_k, norm)
 
 For inference: no call here has a gradient, and an input that requires one is refused while
-gradients are recorded. Everything is enqueued on the current stream; nothing synchronises."""
+gradients are recorded. Everything is enqueued on the current stream; nothing synchronises, there are
+no workspaces. Make the first call on a device outside a capture (it loads the library there)."""
 
 from typing import NamedTuple
 

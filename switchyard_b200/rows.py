@@ -8,8 +8,9 @@ csrc/rows.cu. Beyond the reference, which infers only.
     out = rows.unpermute_rows(y, w, plan)         # [N, H]: every token's rows, weighted and summed
 
 Rows are fp16, bf16 or fp32 with a row of a multiple of 16 bytes, top_k is at most 8. Everything is
-enqueued on the current stream; nothing synchronises, and a plan's addresses are all that a
-captured graph keeps. RuntimeError on any other argument."""
+enqueued on the current stream; nothing synchronises. There are no workspaces: what a captured graph
+keeps are the addresses of its tensors. Make the first call on a device outside a capture (it loads
+the library there). RuntimeError on any other argument."""
 
 from typing import NamedTuple
 
@@ -40,10 +41,13 @@ def _ext():
 
 
 def plan(idx, n_experts):
-    """The plan of idx [N, k] (any integer type): a stable sort of the choices by expert."""
-    if idx.dim() != 2:
-        raise RuntimeError(f"plan: idx must be [tokens, top_k], got {list(idx.shape)}")
-    counts, offsets, token, _, pos_of = _ext().sort_by_expert(idx.to(torch.int32).contiguous(), None, n_experts)
+    """The plan of idx [N, k] (int32 or int64): a stable sort of the choices by expert. Ids outside
+    [0, n_experts) are skipped and leave status 6 (kernels.Ext.device_status)."""
+    if idx.dim() != 2 or idx.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"plan: idx must be int32 or int64 [tokens, top_k], got {idx.dtype} {list(idx.shape)}")
+    if idx.dtype is torch.int64:
+        idx = idx.clamp(-1, n_experts).to(torch.int32)  # (an id past 32 bits must not come back as another)
+    counts, offsets, token, _, pos_of = _ext().sort_by_expert(idx.contiguous(), None, n_experts)
     return SortPlan(counts, offsets, token, pos_of.view(idx.shape))
 
 

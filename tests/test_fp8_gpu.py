@@ -221,6 +221,23 @@ def test_a_row_that_is_not_finite_stays_alone(Q):
     assert torch.isfinite(got[[r for r in range(48) if r not in (3, 41)]]).all()
 
 
+def test_more_than_2_31_elements(Q):
+    """Rows, and rows of results, whose place passes 32 bits: the last rows are those of a small batch."""
+    M, K, N = 1_060_000, 2048, 2056
+    assert M * K > 1 << 31
+    x = torch.randn(64, K, device=DEV, dtype=BF).repeat(M // 64 + 1, 1)[:M].contiguous()
+    w = Q.quantize_weight(torch.randn(2, N, K, device=DEV) * K ** -0.5)
+    x8 = Q.quantize_rows(x)
+    offsets = torch.tensor([0, 1000, M], dtype=torch.int32, device=DEV)
+    del x
+    out = Q.grouped_gemm(x8, w, offsets)
+    last = 1000
+    few8 = Q.Rows8(x8.q[-last:].contiguous(), x8.scale[:, -last:].contiguous())
+    few = Q.grouped_gemm(few8, w, torch.tensor([0, 0, last], dtype=torch.int32, device=DEV))
+    assert same_bits(out[-last:], few)
+    assert same_bits(out[64_000:64_064], out[M - M % 64 - 64:M - M % 64])
+
+
 def layer(N, E, k, H, I, dtype, seed=0):
     g = torch.Generator().manual_seed(seed)
     h = torch.randn(N, H, generator=g).to(dtype).to(DEV)

@@ -264,11 +264,68 @@ def test_a_trained_layer(R, dtype):
         assert (got.double() - ref).norm() <= tol * ref.norm()
 
 
+def test_ids_past_32_bits_are_skipped(R):
+    idx = torch.tensor([[1, 1 << 32], [(1 << 32) + 2, 2], [-(1 << 40), 0]], device=DEV)
+    p = R.plan(idx, 4)
+    assert p.pos_of.tolist() == [[1, -1], [-1, 2], [-1, 0]] and p.counts.tolist() == [1, 1, 1, 0]
+    assert clear_status() == 6
+
+
+def test_more_than_2_31_elements(R):
+    """Rows whose place times their length passes 32 bits."""
+    N, k, H = 140_000, 8, 2048
+    assert N * k * H > 1 << 31
+    idx = (torch.arange(N, device=DEV)[:, None] + torch.arange(k, device=DEV) * 7) % 64
+    p = R.plan(idx.int(), 64)
+    h = torch.randn(N, H, device=DEV, dtype=BF)
+    x = R.permute_rows(h, p)
+    t = torch.tensor([0, 1, 12_345, N - 2, N - 1], device=DEV)
+    assert torch.equal(x[p.pos_of[t].long()], h[t][:, None].expand(-1, k, -1))
+    last = p.token[-3:].long()
+    assert torch.equal(x[-3:], h[last])
+    out = R.unpermute_rows(x, None, p)
+    assert torch.equal(out, 8 * h)  # eight equal rows: exact
+    dy, dw = R._ext().unpermute_rows_grad(h, x, torch.full((N, k), 0.5, device=DEV), p.pos_of, p.offsets)
+    assert torch.equal(dy[p.pos_of[t].long()], (0.5 * h[t])[:, None].expand(-1, k, -1)) and torch.equal(dy[-3:], 0.5 * h[last])
+    sq = (h[t].double() ** 2).sum(1)
+    assert ((dw[t].double() - sq[:, None]).abs() <= 2 * H * 2.0 ** -24 * sq[:, None]).all()
+
+
+def test_a_captured_training_step(R):
+    """Forward and both gradients in one graph, replayed on new values, give the eager step's bits."""
+    N, k, E, H = 50, 4, 16, 128
+    idx, pos, p = setup(R, N, k, E, 0, seed=13)
+    h, w, dout = torch.randn(N, H, device=DEV).to(BF), torch.rand(N, k, device=DEV), torch.randn(N, H, device=DEV).to(BF)
+    def step():
+        a, b = h.detach().requires_grad_(), w.detach().requires_grad_()
+        out = R.unpermute_rows(R.permute_rows(a, p) * 2, b, p)
+        return [out.detach()] + list(torch.autograd.grad(out, (a, b), dout))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for s in range(2):
+        for t in (h, w, dout):
+            t.copy_(torch.randn(t.shape, device=DEV).to(t.dtype))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals(R):
     p = R.plan(torch.zeros(4, 2, dtype=torch.int32, device=DEV), 8)
     h = torch.zeros(4, 64, device=DEV)
     y = torch.zeros(8, 64, device=DEV)
     w = torch.zeros(4, 2, device=DEV)
+    for bad in (torch.zeros(4, 2, device=DEV), torch.zeros(4, 2, dtype=torch.bool, device=DEV), torch.zeros(4, 2, dtype=torch.uint8, device=DEV)):
+        with pytest.raises(RuntimeError, match="int32 or int64"):
+            R.plan(bad, 8)
     for bad in (h.cpu(), h[:3], h.double(), h.int(), h[0], torch.zeros(4, 6, device=DEV)):
         with pytest.raises(RuntimeError):
             R.permute_rows(bad, p)
