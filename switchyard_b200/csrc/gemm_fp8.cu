@@ -224,15 +224,31 @@ __device__ __forceinline__ Tile8 locate_tile8(int t, int& cursor, int E, const i
   return tile;
 }
 
-// silu(g) * u for two columns: the reciprocals of both 1 + exp(-g) come from the one of their
-// product (the special-function unit is what an epilogue waits for). exp and the reciprocal are the
-// approximate ones, within about 2^-21: far inside the 16-bit rounding that follows. exp(-g) is
-// kept below 2^62 so that the product stays finite: below g = -43 sigmoid is taken as 2^-62.
-__device__ __forceinline__ float2 swiglu32(float2 g, float2 u) {
-  constexpr float LOG2E = 1.4426950408889634f;
-  const float d0 = 1.f + exp2_approx(fminf(g.x * -LOG2E, 62.f)), d1 = 1.f + exp2_approx(fminf(g.y * -LOG2E, 62.f));
-  const float r = rcp_approx(d0 * d1);
-  return make_float2(g.x * u.x * (r * d1), g.y * u.y * (r * d0));
+// up <- silu(gate) * up for N pairs of columns. The reciprocals of a pair's 1 + exp(-g) come from the one
+// of their product (the special-function unit is what an epilogue waits for). exp and the
+// reciprocal are the approximate ones, exp within 2^-22 and the rounding of its argument (2^-18 at
+// g = -40): far inside the 16-bit rounding that follows. exp(-g) is kept below 2^62 so that the
+// product stays finite. Where a gate is below that, at -43, the rest of exp(g) is a factor of its own:
+// a thread asks for it once for all its columns (a branch per pair took 2-4 % of a launch).
+template <int N> __device__ __forceinline__ void swiglu_pairs(const uint64_t (&gate)[N], uint64_t (&up)[N]) {
+  constexpr float LOG2E = 1.4426950408889634f, MOST = 62.f;
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float2 g = both(gate[j]), u = both(up[j]);
+    const float x0 = g.x * -LOG2E, x1 = g.y * -LOG2E;
+    const float d0 = 1.f + exp2_approx(fminf(x0, MOST)), d1 = 1.f + exp2_approx(fminf(x1, MOST));
+    const float r = rcp_approx(d0 * d1);
+    up[j] = pair64(make_float2(g.x * (r * d1) * u.x, g.y * (r * d0) * u.y));
+    most = fmaxf(most, fmaxf(x0, x1));
+  }
+  if (__builtin_expect(most > MOST, 0)) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float2 g = both(gate[j]), v = both(up[j]);
+      up[j] = pair64(make_float2(v.x * exp2_approx(fminf(MOST - g.x * -LOG2E, 0.f)), v.y * exp2_approx(fminf(MOST - g.y * -LOG2E, 0.f))));
+    }
+  }
 }
 
 template <typename T, int WR, bool PAIR, bool SWIGLU>
@@ -569,12 +585,12 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         // The row's 128 columns are a block: its largest magnitude over this warp's 64 and, through shared
         // memory, over those of the warp that has the other half. A value is rounded from its product
         // with 448 / m; it comes out of float32 sums, so there are no midpoints to keep.
+        swiglu_pairs(acc[0], acc[1]);
         float top = 0.f;
         bool nan = false;
 #pragma unroll
         for (int j = 0; j < S::COLS / 2; ++j) {
-          const float2 v = swiglu32(both(acc[0][j]), both(acc[1][j]));
-          acc[0][j] = pair64(v);
+          const float2 v = both(acc[1][j]);
           if (col + 2 * j < Nout) {  // Nout is even
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
             nan |= v.x != v.x || v.y != v.y;
@@ -592,7 +608,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         uint32_t o[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float2 a = both(acc[0][2 * j]), b = both(acc[0][2 * j + 1]);
+          const float2 a = both(acc[1][2 * j]), b = both(acc[1][2 * j + 1]);
           o[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a.x * inv, a.y * inv), __NV_SATFINITE, __NV_E4M3) |
                  ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(b.x * inv, b.y * inv), __NV_SATFINITE, __NV_E4M3) << 16);
         }
@@ -600,12 +616,13 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         if (g == 0 && lane < rows)
           args.cscale[(size_t)(col / G8_BLOCK) * args.rows + tile.row0 + trow] = top / 448.f;
       } else if constexpr (SWIGLU) {
+        swiglu_pairs(acc[0], acc[1]);
 #pragma unroll
         for (int c = 0; c < S::COLS; c += 32) {
           uint32_t o[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float2 v = swiglu32(both(acc[0][c / 2 + j]), both(acc[1][c / 2 + j]));
+            const float2 v = both(acc[1][c / 2 + j]);
             o[j] = pack16<T>(v.x, v.y);
           }
           store64(c, o);

@@ -181,6 +181,50 @@ def test_swiglu_straight_to_8_bits(Q, counts, K, N):
     assert torch.equal(less.q[:int(short[-1])].view(torch.uint8), got.q[:int(short[-1])].view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, torch.float8_e4m3fn])
+def test_swiglu_of_very_negative_gates(Q, dtype):
+    """silu far below zero, where sigmoid is e^g: one k block and one term per sum, so gate g and value u are
+    exact and only the epilogue rounds. Its relative error is that of exp2's argument, two roundings of
+    126 at most (2^-17 each, times ln 2), exp2 itself and four products: below 2^-16. Below
+    -87 exp is zero in float32, which leaves |g u| 2^-126. In 8 bits then half a step (2^-4, or 2^-10 scales) and
+    the roundings of test_swiglu_straight_to_8_bits."""
+    gates = torch.tensor([-30.0, -40, -44, -48, -60, -80, -112, -448, -1, 0, 2, 44, 208, 448, -52, -72])
+    N, K, rows = 128, 16, 5
+    xq, wq = torch.zeros(rows, K), torch.zeros(1, 2 * N, K)
+    xq[:, 0] = torch.tensor([1.0, 1, 1, 0.5, 1])
+    wq[0, :N, 0] = gates.repeat(8)
+    wq[0, N:, 0] = torch.tensor([1.0, -448, 0.5, 3]).repeat(32)
+    wq[0, :N, 0][64:] = wq[0, :N, 0][64:].clamp(max=-44)
+    xs = torch.tensor([[1.0, 1, 0.25, 1, 2]])
+    ws = torch.tensor([[[1.0], [2.0 ** 40]]])
+    dev = [t.to(DEV) for t in (xq.to(torch.float8_e4m3fn), xs, wq.to(torch.float8_e4m3fn), ws)]
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    if dtype is HF:
+        dev[3] = torch.tensor([[[1.0], [2.0 ** -4]]], device=DEV)
+    x = xq.double()[:, :1] * xs.double()[0][:, None]
+    g, u = x * wq[0, :N, 0].double(), x * wq[0, N:, 0].double() * float(dev[3][0, 1, 0])
+    ref = g * torch.exp(g) / (1 + torch.exp(g))
+    ref = torch.where(g > 0, g / (1 + torch.exp(-g)), ref) * u
+    d = 2.0 ** -16 * ref.abs() + (g * u).abs() * 2.0 ** -126
+    for rows_ in (slice(0, rows), slice(0, 2), slice(2, 3)):
+        for cols in (slice(0, N), slice(64, N)):  # the second: no gate above -44 * 0.25 in the whole block
+            n = cols.stop - cols.start
+            w = torch.cat([dev[2][:, :N].view(torch.uint8)[:, cols], dev[2][:, N:].view(torch.uint8)[:, cols]], 1).view(torch.float8_e4m3fn)
+            M = rows_.stop - rows_.start
+            got = Q.grouped_gemm(Q.Rows8(dev[0].view(torch.uint8)[rows_].view(torch.float8_e4m3fn), dev[1][:, rows_].contiguous()),
+                                 Q.Weight8(w.contiguous(), dev[3]), (offsets * 0 + torch.tensor([0, M], device=DEV)).int(),
+                                 swiglu=True, dtype=dtype)
+            v, e = ref[rows_, cols], d[rows_, cols]
+            if dtype is torch.float8_e4m3fn:
+                s = got.scale.cpu().double()[0][:, None]
+                e = e + (v.abs() + e) * (2.0 ** -4 + 2.0 ** -21) + 2.0 ** -10 * s
+                assert ((s[:, 0] * 448 - v.abs().amax(1).clamp(min=2.0 ** -96)).abs() <= d[rows_, cols].amax(1) + 2.0 ** -22 * v.abs().amax(1)).all()
+                got = got.q.cpu().double() * s
+            else:
+                e, got = e + rounding(v.abs() + e, dtype), got.cpu().double()
+            assert got.shape == (M, n) and ((got - v).abs() <= e).all(), ((got - v).abs() / e).max()
+
+
 def test_a_rows_bits_do_not_depend_on_its_expert_s_other_rows(Q):
     from switchyard_b200 import kernels
     offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([200], 384, 160, False, 3))
