@@ -51,6 +51,13 @@ def plan(idx, n_experts):
     return SortPlan(counts, offsets, token, pos_of.view(idx.shape))
 
 
+def _incoming(d):
+    """A gradient as the kernels take it. Autograd may hand over any view of its producer's: expanded, strided, or
+    a slice of a flat buffer that starts between 16-byte boundaries."""
+    d = d.contiguous()
+    return d if d.data_ptr() % 16 == 0 else d.clone()
+
+
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, offsets, pos_of):
@@ -61,7 +68,7 @@ class _Permute(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dx):
         pos_of, = ctx.saved_tensors
-        return _ext().unpermute_rows(dx.contiguous(), None, pos_of), None, None
+        return _ext().unpermute_rows(_incoming(dx), None, pos_of), None, None
 
 
 class _Unpermute(torch.autograd.Function):
@@ -75,7 +82,7 @@ class _Unpermute(torch.autograd.Function):
     def backward(ctx, dout):
         y, w, offsets, pos_of = ctx.saved_tensors
         need_dy, need_dw = ctx.needs_input_grad[:2]
-        dy, dw = _ext().unpermute_rows_grad(dout.contiguous(), y, w, pos_of, offsets, need_dy, need_dw)
+        dy, dw = _ext().unpermute_rows_grad(_incoming(dout), y, w, pos_of, offsets, need_dy, need_dw)
         return dy, dw, None, None
 
 

@@ -173,6 +173,25 @@ def test_strided_inputs_and_expanded_gradients(R):
     assert ((dw.cpu().double() - rows_sum).abs() <= sum_bound(rows_sum, mag, 72, F32)).all()
 
 
+def test_gradients_that_start_between_16_byte_boundaries(R):
+    """A flat torch.cat hands its inputs slices of one gradient, which may start anywhere."""
+    from switchyard_b200 import kernels
+    idx, pos, p = setup(R, 9, 2, 4, 0, seed=12)
+    g = torch.Generator().manual_seed(3)
+    h, one = torch.randn(9, 64, generator=g).to(DEV).requires_grad_(), torch.zeros(1, device=DEV, requires_grad=True)
+    w = torch.rand(9, 2, generator=g).to(DEV).requires_grad_()
+    x = R.permute_rows(h, p)
+    d = torch.randn(1 + x.numel(), generator=g).to(DEV)
+    dh, = torch.autograd.grad(torch.cat([one, x.flatten()]), h, d)
+    assert torch.equal(dh, kernels.ext().unpermute_rows(d[1:].clone().view(x.shape), None, p.pos_of))
+    y = x.detach().requires_grad_()
+    out = R.unpermute_rows(y, w, p)
+    d = d[:1 + out.numel()].clone()
+    dy, dw = torch.autograd.grad(torch.cat([one, out.flatten()]), (y, w), d)
+    want = kernels.ext().unpermute_rows_grad(d[1:].clone().view(out.shape), y.detach(), w.detach(), p.pos_of, p.offsets)
+    assert torch.equal(dy, want[0]) and torch.equal(dw, want[1])
+
+
 def test_values_that_are_not_finite_stay_in_their_token(R):
     idx, pos, p = setup(R, 9, 2, 8, 0, seed=4)
     y = torch.ones(18, 16, dtype=BF)
