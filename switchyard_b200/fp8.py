@@ -57,8 +57,8 @@ def refuse(name, *weights):
         raise RuntimeError(f"{name}: 8-bit experts (fp8.Weight8) are for one GPU; pass the 16-bit stacks")
 
 
-def _no_grad(name, t):
-    if t is not None and t.requires_grad and torch.is_grad_enabled():
+def _no_grad(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
@@ -87,7 +87,7 @@ def grouped_gemm(x, w, offsets, swiglu=False, scale=None, dtype=torch.bfloat16):
     (bf16 or fp16). dtype float8_e4m3fn, with swiglu: the result as Rows8 for the next product, quantised
     where it is computed (scale = m / 448 and q = e4m3(v * (448 / m)) of the float32 values). Rows of no
     expert are zero. A row's bits depend on nothing but the row and its expert's weights."""
-    _no_grad("grouped_gemm", scale)
+    _no_grad("grouped_gemm", x.q, x.scale, w.q, w.scale, scale)
     out = _rows._ext().grouped_gemm_fp8(x.q, x.scale, w.q, w.scale, offsets, swiglu, scale, dtype)
     return Rows8(*out) if dtype is torch.float8_e4m3fn else out
 

@@ -393,6 +393,8 @@ class Ext:
             raise RuntimeError(f"quantize_rows: x must be [tokens, hidden], got {list(x.shape)}")
         N, H = x.shape
         k = experts = 1
+        if (pos_of is None) != (offsets is None):
+            raise RuntimeError("quantize_rows: pos_of and offsets come together")
         if pos_of is not None:
             n, k = _check_places(pos_of, offsets, dev, "quantize_rows")
             experts = offsets.numel() - 1
@@ -401,7 +403,7 @@ class Ext:
         q = torch.empty((N * k, H), dtype=torch.float8_e4m3fn, device=x.device)
         scale = torch.empty(((H + 127) // 128, N * k), dtype=torch.float32, device=x.device)
         with _Device(dev) as stream:
-            rc = self.lib.sy_quantize_rows(x.data_ptr(), _ptr(pos_of), _ptr(offsets) if pos_of is not None else None, N, k,
+            rc = self.lib.sy_quantize_rows(x.data_ptr(), _ptr(pos_of), _ptr(offsets), N, k,
                                            experts, H, code, q.data_ptr(), scale.data_ptr(), stream)
         _lib.check(rc, "quantize_rows")
         return q, scale

@@ -375,6 +375,7 @@ def test_streams_and_graphs(Q):
 
 def test_refusals(Q):
     from switchyard_b200 import kernels
+    from switchyard_b200.rows import plan
     offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([4, 4], 128, 64, False, 1))
     x, w = Q.Rows8(xq, xs), Q.Weight8(wq, ws)
     bad = [dict(x=x._replace(scale=xs.t())), dict(x=x._replace(q=xq.float())), dict(w=w._replace(scale=ws[:1])),
@@ -396,6 +397,10 @@ def test_refusals(Q):
             Q.quantize_weight(t, halves)
     with pytest.raises(RuntimeError, match="multiple of 16"):  # experts of width 136: 16-bit only
         Q.quantize_weight(layer(1, 8, 2, 256, 136, BF)[3])
+    p = plan(torch.zeros(4, 2, dtype=torch.int32, device=DEV), 8)
+    for places_ in ((p.pos_of, None), (None, p.offsets), (p.pos_of[:3], p.offsets), (p.pos_of.long(), p.offsets)):
+        with pytest.raises(RuntimeError, match="quantize_rows"):
+            kernels.ext().quantize_rows(torch.zeros(4, 32, device=DEV), *places_)
     leaf = torch.zeros(4, 32, device=DEV, requires_grad=True)
     with pytest.raises(RuntimeError, match="no gradient"):
         Q.quantize_rows(leaf)

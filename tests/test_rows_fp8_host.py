@@ -87,6 +87,23 @@ def test_tensors_on_the_host_are_refused(lib):
             call()
 
 
+def test_8_bit_calls_refuse_inputs_that_require_a_gradient(lib):
+    from switchyard_b200 import fp8
+    t = lambda *shape, grad=False: torch.zeros(*shape, requires_grad=grad)
+    x, w = fp8.Rows8(t(4, 128), t(1, 4)), fp8.Weight8(t(1, 8, 128), t(1, 1, 1))
+    offsets = torch.zeros(2, dtype=torch.int32)
+    for changed in (dict(x=x._replace(scale=t(1, 4, grad=True))), dict(w=w._replace(scale=t(1, 1, 1, grad=True))),
+                    dict(scale=t(4, grad=True))):
+        args = {**dict(x=x, w=w, offsets=offsets), **changed}
+        with pytest.raises(RuntimeError, match="no gradient"):
+            fp8.grouped_gemm(**args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):  # without recording: the next check
+            fp8.grouped_gemm(**args)
+    for call in (fp8.quantize_rows, fp8.quantize_weight):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(t(4, 32, grad=True))
+
+
 def test_the_plain_quantiser_is_torchs_e4m3(lib):
     """nearest8 against torch's own conversion on every 16-bit value it can take, ties included."""
     v = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(torch.float16).float()
