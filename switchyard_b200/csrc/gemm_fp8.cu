@@ -47,6 +47,7 @@ constexpr int G8_SLOTS = 16;                     // k blocks whose scales are in
 constexpr int G8_OUT_PITCH = 64 + 16;             // bytes per staged row of results: 32 columns, off the banks of the next
 constexpr int G8_SLOT = G8_XR + 8;               // floats: the rows' scales, then the weights' two
 constexpr int G8_HELPERS = 4;                    // warps before the promoters: TMA, two for MMA, scales
+constexpr int G8_MOST = 0x7fff0000;              // rows and k: a tile's or a block's end is still a 32-bit number
 constexpr int G8_RING_BYTES = 192 * 1024;
 constexpr int G8_SMEM = G8_RING_BYTES + 1024;    // room to align the ring to 1024
 
@@ -388,9 +389,11 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         }
       }
       // The copies already issued land before the block can exit, whoever gave up on a wait. (PAIR: the other
-      // CTA's count on the leader's barriers too, and it does not leave before the leader.)
-      if (cr == 0 && lane == 0)
-        for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(&full_bar[j % STAGES], (j / STAGES) & 1, 10000000ull);
+      // CTA's count on the leader's barriers, and it does not leave before the leader; what it waits for
+      // itself is the leader's last words on its own barriers.)
+      if (lane == 0)
+        for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j)
+          mbar_wait(cr == 0 ? &full_bar[j % STAGES] : &empty_bar[j % STAGES], (j / STAGES) & 1, 10000000ull);
     } else if (warp <= 2) {
       // -------------------------------------------------------------- MMA issuers (PAIR: the leader's, for both CTAs)
       // Two warps take the k blocks in turn: a wait costs its warp 100 to 250 clocks even when there is
@@ -746,9 +749,11 @@ extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const vo
                                    const int32_t* offsets, int n_experts, int rows, int n_out, int k_dim, int swiglu,
                                    const void* scale, void* C, float* c_scale, int dtype, int tile, void* stream) {
   using namespace sy;
-  SY_REQUIRE(rows >= 0 && n_experts >= 1 && n_experts <= G8_MAX_E, "grouped_gemm_fp8: 1..%d experts (got %d)", G8_MAX_E,
+  SY_REQUIRE(rows >= 0 && rows <= G8_MOST, "grouped_gemm_fp8: 0..%d rows (got %d)", G8_MOST, rows);
+  SY_REQUIRE(n_experts >= 1 && n_experts <= G8_MAX_E, "grouped_gemm_fp8: 1..%d experts (got %d)", G8_MAX_E,
              n_experts);
-  SY_REQUIRE(k_dim > 0 && k_dim % 16 == 0, "grouped_gemm_fp8: k_dim must be a multiple of 16 (got %d)", k_dim);
+  SY_REQUIRE(k_dim > 0 && k_dim <= G8_MOST && k_dim % 16 == 0,
+             "grouped_gemm_fp8: k_dim must be a multiple of 16, at most %d (got %d)", G8_MOST, k_dim);
   SY_REQUIRE(n_out > 0 && n_out % 8 == 0, "grouped_gemm_fp8: n_out must be a multiple of 8 (got %d)", n_out);
   SY_REQUIRE(!(swiglu && scale), "grouped_gemm_fp8: swiglu and scale are separate epilogues");
   SY_REQUIRE(c_scale || dtype == SY_DTYPE_F16 || dtype == SY_DTYPE_BF16, "grouped_gemm_fp8: dtype must be f16 or bf16");

@@ -220,8 +220,9 @@ extern "C" int sy_quantize_rows(const void* x, const int32_t* pos_of, const int3
              "quantize_rows: dtype must be f16, bf16 or f32");
   SY_REQUIRE(n_tokens >= 0 && top_k >= 1 && top_k <= ROWS_MAX_K, "quantize_rows: top_k must be 1..%d (got %d)", ROWS_MAX_K,
              top_k);
-  SY_REQUIRE(n_tokens <= 0x7fffffff / top_k, "quantize_rows: more than 2^31 rows");
-  SY_REQUIRE(hidden > 0 && hidden % 16 == 0, "quantize_rows: hidden must be a multiple of 16 (got %d)", hidden);
+  SY_REQUIRE(n_tokens <= ROWS_MOST / top_k, "quantize_rows: more than 2^31 - 256 rows");
+  SY_REQUIRE(hidden > 0 && hidden <= WIDTH_MOST && hidden % 16 == 0,
+             "quantize_rows: hidden must be a multiple of 16, at most %d (got %d)", WIDTH_MOST, hidden);
   if (n_tokens == 0) return SY_OK;
   SY_REQUIRE(pos_of || top_k == 1, "quantize_rows: rows kept in place have one place each");
   SY_REQUIRE(!pos_of || n_experts >= 1, "quantize_rows: at least one expert (got %d)", n_experts);
@@ -241,7 +242,8 @@ extern "C" int sy_quantize_weight(const void* w, int n_mats, int n_rows, int k_d
              "quantize_weight: dtype must be f16, bf16 or f32");
   SY_REQUIRE(n_mats >= 0 && n_mats <= 65535, "quantize_weight: at most 65535 matrices (got %d)", n_mats);
   SY_REQUIRE(n_rows > 0 && n_rows <= 65535 * Q8_BLOCK, "quantize_weight: 1..%d rows (got %d)", 65535 * Q8_BLOCK, n_rows);
-  SY_REQUIRE(k_dim > 0 && k_dim % 16 == 0, "quantize_weight: k_dim must be a multiple of 16 (got %d)", k_dim);
+  SY_REQUIRE(k_dim > 0 && k_dim <= WIDTH_MOST && k_dim % 16 == 0,
+             "quantize_weight: k_dim must be a multiple of 16, at most %d (got %d)", WIDTH_MOST, k_dim);
   if (n_mats == 0) return SY_OK;
   SY_REQUIRE(w && q && scale, "quantize_weight: null pointer");
   SY_REQUIRE((uintptr_t)w % 16 == 0 && (uintptr_t)q % 16 == 0, "quantize_weight: w and q must be 16-byte aligned");

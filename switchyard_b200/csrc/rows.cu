@@ -193,10 +193,10 @@ static int rows_check(const char* name, int n_tokens, int top_k, int hidden, int
   SY_REQUIRE(dtype == SY_DTYPE_F16 || dtype == SY_DTYPE_BF16 || dtype == SY_DTYPE_F32, "%s: dtype must be f16, bf16 or f32",
              name);
   SY_REQUIRE(n_tokens >= 0 && top_k >= 1 && top_k <= ROWS_MAX_K, "%s: top_k must be 1..%d (got %d)", name, ROWS_MAX_K, top_k);
-  SY_REQUIRE(n_tokens <= 0x7fffffff / top_k, "%s: more than 2^31 rows", name);
+  SY_REQUIRE(n_tokens <= ROWS_MOST / top_k, "%s: more than 2^31 - 256 rows", name);
   const int per_vec = dtype == SY_DTYPE_F32 ? 4 : 8;
-  SY_REQUIRE(hidden > 0 && hidden % per_vec == 0, "%s: hidden must be a multiple of %d in this type (got %d)", name, per_vec,
-             hidden);
+  SY_REQUIRE(hidden > 0 && hidden <= WIDTH_MOST && hidden % per_vec == 0,
+             "%s: hidden must be a multiple of %d in this type, at most %d (got %d)", name, per_vec, WIDTH_MOST, hidden);
   *vecs = hidden / per_vec;
   return SY_OK;
 }

@@ -5,6 +5,8 @@
 namespace sy {
 
 constexpr int ROWS_MAX_K = 8;  // most choices per token, as in route and combine
+constexpr int ROWS_MOST = 0x7fffff00;   // rows, so that a block's last token is still a 32-bit number
+constexpr int WIDTH_MOST = 0x7fff0000;  // columns, likewise
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }

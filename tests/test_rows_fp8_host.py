@@ -39,6 +39,11 @@ def test_row_operators_refuse(lib):
     refused(lib, lib.sy_unpermute_rows(P, None, 0, None, 4, 2, 64, 1, P, None), b"null")
     refused(lib, lib.sy_unpermute_rows_grad(P, P, P, 0, P, P, 4, 2, 8, 64, 1, P, P, None), b"weights")
     refused(lib, lib.sy_unpermute_rows_grad(P, None, P, 1, P, P, 4, 2, 8, 64, 1, P, P, None), b"null")
+    # the largest sizes: a block's last token and a row's last column are 32-bit numbers
+    most = 0x7fffffff
+    refused(lib, lib.sy_permute_rows(P, P, P, most, 1, 8, 64, 1, P, None), b"2^31")
+    refused(lib, lib.sy_unpermute_rows(P, None, 1, P, most - 100, 1, 64, 1, P, None), b"2^31")
+    refused(lib, lib.sy_unpermute_rows_grad(P, P, P, 1, P, P, 1, 1, 8, most - 7, 1, P, P, None), b"at most")
     # nothing to do: no pointer is needed
     assert lib.sy_permute_rows(None, None, None, 0, 2, 8, 64, 1, None, None) == 0
     assert lib.sy_unpermute_rows(None, None, 0, None, 0, 2, 64, 1, None, None) == 0
@@ -67,6 +72,12 @@ def test_quantisers_and_the_product_refuse(lib):
     refused(lib, lib.sy_grouped_gemm_fp8(*args(cs=P, sw=1, tile=1)), b"wide")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(x=None)), b"null")
     refused(lib, lib.sy_grouped_gemm_fp8(*args(x=ctypes.c_void_p(8))), b"aligned")
+    most = 0x7ffffff0  # the largest multiple of 16
+    refused(lib, lib.sy_quantize_rows(P, None, None, most, 1, 0, 64, 1, P, P, None), b"2^31")
+    refused(lib, lib.sy_quantize_rows(P, None, None, 1, 1, 0, most, 1, P, P, None), b"at most")
+    refused(lib, lib.sy_quantize_weight(P, 1, 8, most, 1, P, P, None), b"at most")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(rows=most)), b"rows")
+    refused(lib, lib.sy_grouped_gemm_fp8(*args(k=most)), b"at most")
     assert lib.sy_grouped_gemm_fp8(*args(rows=0, x=None)) == 0
     refused(lib, lib.sy_sort_by_expert(P, P, 8, 2, 8, 0, P, P, P, None, P, None, 0, None), b"null")
 
