@@ -240,17 +240,21 @@ __device__ __forceinline__ Tile8 locate_tile8(int t, int& cursor, int E, const i
 // reciprocal are the approximate ones, exp within 2^-22 and the rounding of its argument (2^-18 at
 // g = -40): far inside the 16-bit rounding that follows. exp(-g) is kept below 2^62 so that the
 // product stays finite. Where a gate is below that, at -43, the rest of exp(g) is a factor of its own:
-// a thread asks for it once for all its columns (a branch per pair took 2-4 % of a launch).
-template <int N> __device__ __forceinline__ void swiglu_pairs(const uint64_t (&gate)[N], uint64_t (&up)[N]) {
+// a thread asks for it once for all its columns (a branch per pair took 2-4 % of a launch). The bits are
+// the same with PACKED products or single ones: 16-bit results are 1-2 % faster with the packed (65,536
+// rows 257 -> 253 us), 8-bit results with the single ones (257, packed 260).
+template <bool PACKED, int N> __device__ __forceinline__ void swiglu_pairs(const uint64_t (&gate)[N], uint64_t (&up)[N]) {
   constexpr float LOG2E = 1.4426950408889634f, MOST = 62.f;
   float most = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const float2 g = both(gate[j]), u = both(up[j]);
-    const float x0 = g.x * -LOG2E, x1 = g.y * -LOG2E;
+    const float2 x = PACKED ? both(mul2(gate[j], twice(-LOG2E))) : make_float2(g.x * -LOG2E, g.y * -LOG2E);
+    const float x0 = x.x, x1 = x.y;
     const float d0 = 1.f + exp2_approx(fminf(x0, MOST)), d1 = 1.f + exp2_approx(fminf(x1, MOST));
     const float r = rcp_approx(d0 * d1);
-    up[j] = pair64(make_float2(g.x * (r * d1) * u.x, g.y * (r * d0) * u.y));
+    if (PACKED) up[j] = mul2(mul2(gate[j], mul2(pair64(make_float2(d1, d0)), twice(r))), up[j]);
+    else up[j] = pair64(make_float2(g.x * (r * d1) * u.x, g.y * (r * d0) * u.y));
     most = fmaxf(most, fmaxf(x0, x1));
   }
   if (__builtin_expect(most > MOST, 0)) {
@@ -600,7 +604,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         // The row's 128 columns are a block: its largest magnitude over this warp's 64 and, through shared
         // memory, over those of the warp that has the other half. A value is rounded from its product
         // with 448 / m; it comes out of float32 sums, so there are no midpoints to keep.
-        swiglu_pairs(acc[0], acc[1]);
+        swiglu_pairs<!OUT8>(acc[0], acc[1]);
         float top = 0.f;
         if (col + S::COLS <= Nout) {
 #pragma unroll
@@ -634,7 +638,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         if (g == 0 && lane < rows)
           args.cscale[(size_t)(col / G8_BLOCK) * args.rows + tile.row0 + trow] = top / 448.f;
       } else if constexpr (SWIGLU) {
-        swiglu_pairs(acc[0], acc[1]);
+        swiglu_pairs<!OUT8>(acc[0], acc[1]);
 #pragma unroll
         for (int c = 0; c < S::COLS; c += 32) {
           uint32_t o[16];
