@@ -598,6 +598,33 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         }
         __syncwarp();
       };
+      // The same with 128 bytes of a row, half of the rows at a time: whole lines, where there are so many results
+      // that the epilogues' writes are what waits (65,536 rows by 2048 columns, k 1024: 175 -> 167 us of
+      // the wide tile, 170 -> 164 of the pair's; 8 rows per expert 26.4 -> 26.7; SwiGLU's half as many
+      // results were no faster for it).
+      auto store128 = [&](int c, const uint32_t (&o)[32]) {
+        constexpr int PART = 16 / sizeof(T), PITCH = 128 + 16;
+        static_assert(16 * PITCH <= sizeof(s_out[0]), "staging");
+        unsigned char* half = s_out[warp - G8_HELPERS];
+        const int part = lane & 7;
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += 16) {
+          if ((lane & 16) == r0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(half + (lane & 15) * PITCH + i * 16) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(half + r * PITCH + part * 16);
+            if (r0 + r < rows && col + c + part * PART < Nout)
+              *reinterpret_cast<uint4*>(to + (size_t)(r0 + r) * Nout + c + part * PART) = v;
+          }
+          __syncwarp();
+        }
+      };
       if constexpr (OUT8) {
         // (Every operation per value counts: with two for the maximum and one for NaN, not two and three and
         // a bound, and packed products, a launch of 65,536 rows went from 276 to 260 us.)
@@ -648,6 +675,17 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
             o[j] = pack16<T>(v.x, v.y);
           }
           store64(c, o);
+        }
+      } else if constexpr (S::COLS == 64) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 v = both(acc[h][j]);
+            o[j] = pack16<T>(v.x * row_scale, v.y * row_scale);
+          }
+          store128(h * (WR / 2), o);
         }
       } else {
 #pragma unroll
