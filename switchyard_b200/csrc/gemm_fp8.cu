@@ -784,20 +784,23 @@ static int dispatch8(const Gemm8Args& a, int tile, const void* x, const void* w,
 
 // Which tile a batch gets; the bits are the same. Measured on a B200 with the benchmark's layer (64 experts,
 // gate and up 2048 x 2048 with SwiGLU, down 2048 x 1024), us for the narrow / wide / pair tile:
-//   1 token     gate-up 10.3 / 13.0 / 14.4    down  6.9 /  8.2 /  9.6   (wide: fewer tiles than SMs)
-//   8 tokens            34.9 / 37.2 / 46.8         21.7 / 21.8 / 29.8
-//   64 tokens           48.8 / 51.1 / 66.1         29.1 / 27.7 / 39.3
-//   512 tokens          53.1 / 54.1 / 69.3         30.9 / 30.7 / 42.8   (64 rows per expert)
-//   1024 tokens         75.6 / 67.5 / 73.6         45.1 / 40.8 / 47.8
-//   4096 tokens          204 /  172 /  172          126 /  106 /  110
-//   8192 tokens          380 /  313 /  299                              (1024 rows per expert)
-// So: pairs from 768 rows per expert; the wide tile from 64, and for plain products below that too where
-// it gives every SM a tile; else the narrow one, which SwiGLU's shorter rows of results suit.
+//   1 token     gate-up 11.0 / 14.4 / 14.2    down  6.9 /  8.2 /  9.6   (wide: fewer tiles than SMs)
+//   8 tokens            37.0 / 37.1 / 45.5         21.6 / 21.0 / 28.6
+//   16 tokens           43.2 / 42.3
+//   64 tokens           51.2 / 50.0 / 64.7         29.4 / 26.7 / 37.6   (gate-up on another card 48.0 / 49.9;
+//                       31.4 / 28.9 with half the k, 29.9 / 27.6 with half the columns)
+//   512 tokens          53.9 / 50.7 / 67.6         31.0 / 26.9 / 39.3   (64 rows per expert)
+//   1024 tokens         75.8 / 67.4 / 72.4         45.0 / 39.2 / 43.8
+//   4096 tokens          204 /  167 /  168          118 /  100 /  102
+//   8192 tokens          372 /  305 /  303          219 /  184 /  183   (1024 rows per expert)
+// So: pairs from 768 rows per expert; the wide tile where it gives every SM a tile, SwiGLU only beyond a
+// row per expert; else the narrow one, which has twice the tiles.
 static int choose_tile8(int rows, int experts, int n_out, bool swiglu, int sms) {
   if (rows >= 768LL * experts) return 3;
   if (rows > 64LL * experts) return 2;
-  const long long wide = (long long)(rows < experts ? rows : experts) * ((n_out + 255) / 256);
-  return !swiglu && wide >= sms ? 2 : 1;
+  const long long cols = swiglu ? 128 : 256;
+  const long long wide = (long long)(rows < experts ? rows : experts) * ((n_out + cols - 1) / cols);
+  return wide >= sms && (!swiglu || rows > experts) ? 2 : 1;
 }
 
 }  // namespace sy

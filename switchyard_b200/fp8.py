@@ -92,27 +92,15 @@ def grouped_gemm(x, w, offsets, swiglu=False, scale=None, dtype=torch.bfloat16):
     return Rows8(*out) if dtype is torch.float8_e4m3fn else out
 
 
-# "auto" is "gemv" up to this many rows per expert on average, where the product's narrow tile applies. The
-# benchmark's layer, graph replays, us for gemv / gemm: 8 tokens 87.5 / 86.1, 64 107 / 109, 256 115 / 117,
-# 512 (64 rows per expert) 122 / 119, 1024 155 / 150, 4096 413 / 381, 8192 732 / 685.
-AUTO_GEMV_MAX_MEAN_ROWS = 64
-
-
 def sorted_experts(h, plan, wsorted, gate_up, down, mode="auto"):
     """The expert FFN on 8-bit weights for a sorted batch: rows quantised into expert order, gate/up
-    product with SwiGLU, its result in 8 bits, down product times the router weights wsorted. Mode "gemv"
-    (decode): the SwiGLU result is rounded to h's dtype and quantised by a launch of its own; "gemm" (and
-    "cublas"): quantised from float32 where it is computed. The two are separate contracts, within each a
-    row's bits do not depend on the batch; "auto" chooses from the mean rows per expert.
-    Returns y [N*k, H] in h's dtype, for combine."""
+    product with SwiGLU, its float32 result quantised where it is computed, down product times the router
+    weights wsorted. There is one path for every batch (a result in h's dtype quantised by a launch of its own
+    took as long at one token and 5-9 % longer from 8 tokens on): `mode` is checked and chooses nothing,
+    and a row's bits do not depend on the batch. Returns y [N*k, H] in h's dtype, for combine."""
     if mode not in ("auto", "gemv", "gemm", "cublas"):
         raise RuntimeError(f"sorted_experts: unknown mode {mode!r}")
     if not (isinstance(gate_up, Weight8) and isinstance(down, Weight8)):
         raise RuntimeError("sorted_experts: gate_up and down must both be 8-bit (fp8.Weight8) or both 16-bit")
-    few = plan.pos_of.numel() <= AUTO_GEMV_MAX_MEAN_ROWS * gate_up.q.shape[0] if mode == "auto" else mode == "gemv"
-    x = quantize_rows(h, plan)
-    if few:
-        act = quantize_rows(grouped_gemm(x, gate_up, plan.offsets, swiglu=True, dtype=h.dtype))
-    else:
-        act = grouped_gemm(x, gate_up, plan.offsets, swiglu=True, dtype=torch.float8_e4m3fn)
+    act = grouped_gemm(quantize_rows(h, plan), gate_up, plan.offsets, swiglu=True, dtype=torch.float8_e4m3fn)
     return grouped_gemm(act, down, plan.offsets, scale=wsorted, dtype=h.dtype)

@@ -17,7 +17,7 @@ Differences a caller can observe:
     the largest expert's row count, so the layer never synchronises;
   * `experts`, `moe_layer` and `GraphedLayer` also take 8-bit expert weights (`fp8.Weight8` for both
     gate_up and down): the rows are then quantised on their way into expert order and both
-    products run in e4m3 (`fp8.sorted_experts` says what `mode` chooses there);
+    products run in e4m3 (`fp8.sorted_experts`; `mode` chooses nothing there);
   * `route_fused` computes the router logits inside the routing launch instead of calling the
     library GEMM. It is not what `moe_layer` uses unless SWITCHYARD_FUSED_ROUTER=1 (or
     `route_and_sort(..., fused=True)`): measured on a B200 the library GEMM followed by the

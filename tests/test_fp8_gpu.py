@@ -295,9 +295,9 @@ def layer(N, E, k, H, I, dtype, seed=0):
                                              (333, 64, 8, 256, 144, BF), (2100, 8, 4, 256, 128, BF), (0, 8, 2, 128, 64, BF)])
 def test_the_layer_on_8_bit_experts(Q, N, E, k, H, I, dtype):
     """moe_layer with Weight8 experts: route, sort, quantise into expert order, product with SwiGLU and
-    its result to 8 bits ("gemv": by a launch of its own, "gemm": where it is computed), product
-    with router weights, combine: the bits of the operators called one by one, with a residual and
-    through GraphedLayer too; and near the 16-bit layer."""
+    its result to 8 bits where it is computed, product with router weights, combine: the bits of the
+    operators called one by one in every mode, with a residual and through GraphedLayer too; and
+    near the 16-bit layer."""
     from switchyard_b200 import kernels, rows
     h, router, gate_up, down = layer(N, E, k, H, I, dtype)
     gu8, dn8 = Q.quantize_weight(gate_up, halves=2), Q.quantize_weight(down)
@@ -308,12 +308,13 @@ def test_the_layer_on_8_bit_experts(Q, N, E, k, H, I, dtype):
     idx, w, counts, offsets, token, wsorted, pos_of = kernels.route_and_sort(h, router, k, False)
     plan = rows.SortPlan(counts, offsets, token, pos_of.view(N, k))
     x8 = Q.quantize_rows(h, plan)
-    acts = {"gemv": Q.quantize_rows(Q.grouped_gemm(x8, gu8, offsets, swiglu=True, dtype=dtype)),
-            "gemm": Q.grouped_gemm(x8, gu8, offsets, swiglu=True, dtype=torch.float8_e4m3fn)}
-    for mode, act in acts.items():
-        y = Q.grouped_gemm(act, dn8, offsets, scale=wsorted, dtype=dtype)
-        assert torch.equal(kernels.moe_layer(h, router, gu8, dn8, k, False, mode), kernels.ext().combine(y, pos_of, idx, N))
-    assert torch.equal(out, kernels.moe_layer(h, router, gu8, dn8, k, False, "gemv" if N * k <= 64 * E else "gemm"))
+    act = Q.grouped_gemm(x8, gu8, offsets, swiglu=True, dtype=torch.float8_e4m3fn)
+    y = Q.grouped_gemm(act, dn8, offsets, scale=wsorted, dtype=dtype)
+    assert torch.equal(out, kernels.ext().combine(y, pos_of, idx, N))
+    for mode in ("gemv", "gemm", "cublas"):
+        assert torch.equal(kernels.moe_layer(h, router, gu8, dn8, k, False, mode), out)
+    some = torch.arange(0, N, 3, device=DEV)  # a row's bits do not depend on the batch
+    assert torch.equal(kernels.experts(h[some], idx[some], w[some], gu8, dn8), out[some])
     assert torch.equal(kernels.experts(h, idx, w, gu8, dn8), out)
     x = torch.randn_like(h)
     assert torch.equal(kernels.moe_layer(h, router, gu8, dn8, k, False, residual=x), x + out)
