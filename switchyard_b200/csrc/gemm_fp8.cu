@@ -20,12 +20,13 @@
 // gate rows and the up rows of the same columns. A thread takes the same quarter of the columns out
 // of either half, so that it finds a gate value and its up value in its own registers.
 //
-// What bounds it. Few rows per expert: the weights' way from HBM (64 tokens, 268 MB of gate and up: 48 us,
-// 5.6 TB/s). Many rows: the chain of one partial product, MMA - barrier - promotion - barrier - MMA,
-// against two buffers (950 clocks a block of 256 columns and two CTAs, where the MMAs alone take 512);
-// and, run for seconds, the GPU's power: 8192 tokens take 299 us in a burst at 1.65 GHz, 356 us at
-// 1.44 GHz and 990 W, of which the promotion's multiply-adds are 67 us. (The library's 8-bit product
-// of the same size, one scale per matrix, no experts, no SwiGLU, takes 246 us at the same power.)
+// What bounds it. Few rows per expert: the weights' way from HBM (64 tokens, 268 MB of gate and up: 49 us,
+// 5.5 TB/s), and a last round of tiles, 5 us however few they are. Many rows: a block of 256 columns over
+// two CTAs takes 0.43 us where the MMAs alone take 0.27, with shared memory busy for two thirds of it (by its bytes: 64 KB at 128 a clock), and
+// the epilogues are a quarter of a launch of 16 blocks a tile; and, run for seconds, the GPU's power: 8192
+// tokens take 292 us in a burst, 341-350 us at 1.45 GHz and 990 W, of which the promotion's multiply-adds
+// were 67 us. (The library's 8-bit product of the same size, one scale per matrix, no experts, no
+// SwiGLU, takes 246 us at the same power.)
 #include <cuda.h>
 #include <cuda_fp8.h>
 
