@@ -58,6 +58,13 @@ def _incoming(d):
     return d if d.data_ptr() % 16 == 0 else d.clone()
 
 
+def _once(backward):
+    """once_differentiable, entered only where a graph of the gradient is being recorded: its own guards are 5 us of
+    an 88 us pass forward and back."""
+    guarded = once_differentiable(backward)
+    return lambda ctx, *grads: guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, offsets, pos_of):
@@ -65,7 +72,7 @@ class _Permute(torch.autograd.Function):
         return _ext().permute_rows(h, pos_of, offsets)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dx):
         pos_of, = ctx.saved_tensors
         return _ext().unpermute_rows(_incoming(dx), None, pos_of), None, None
@@ -78,7 +85,7 @@ class _Unpermute(torch.autograd.Function):
         return _ext().unpermute_rows(y, w, pos_of)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         y, w, offsets, pos_of = ctx.saved_tensors
         need_dy, need_dw = ctx.needs_input_grad[:2]
