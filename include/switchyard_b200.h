@@ -292,7 +292,7 @@ int sy_quantize_weight(const void* w, int n_mats, int n_rows, int k_dim, int dty
  * c_scale = m / 448 and C = e4m3(v * (448 / m)) of the float32 values v; dtype is not looked at.
  * offsets int32 [n_experts + 1]; values outside [0, rows] are clamped, rows of no expert are set to
  * zero. A row's bits do not depend on the other rows of its expert or on the tile.
- * tile: 0 = chosen from the mean rows per expert; 1 = 128 rows x 128 weight rows (not with c_scale),
+ * tile: 0 = chosen from the mean rows per expert; 1 = 32 rows x 128 weight rows (256 with c_scale),
  * 2 = 128 x 256, 3 = 256 x 256 over a pair of CTAs. k_dim % 16 == 0, n_out % 8 == 0, n_experts <= 256, x, w and C
  * 16-byte aligned. */
 int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const void* w, const float* w_scale, const int32_t* offsets,

@@ -9,24 +9,30 @@
 // Float32 scales cannot ride in the tensor core, so the inner sums of each block of 128 (four
 // tcgen05.mma of k = 32) go to tensor memory on their own, and eight warps multiply them by the two
 // scales and add them up in float32 registers (the promotion) while the next block is being
-// multiplied: tensor memory holds two such partial products of 256 columns, or four of 128. A
-// thread owns a row of the tile and a quarter of its columns. Both scales are the same for all of a
-// thread's columns of one weight block, so a value costs half a packed multiply-add.
+// multiplied: tensor memory holds two such partial products of 256 columns, or four smaller ones.
 //
 // Warps: 0 TMA producer, 1-2 MMA issuers, 3 scales, 4-11 promotion and epilogue.
 // Tiles as in gemm.cu: numbered on the device from `offsets`, expert-major, dealt round-robin to
-// a persistent grid. Token rows are the MMA's M operand (128, or 256 over a pair of CTAs), weight
-// rows its N operand, in two halves of WR / 2 (a TMA box each): consecutive rows, or with SwiGLU the
-// gate rows and the up rows of the same columns. A thread takes the same quarter of the columns out
-// of either half, so that it finds a gate value and its up value in its own registers.
+// a persistent grid. Weight rows come in two halves (a TMA box each): consecutive rows, or with SwiGLU
+// the gate rows and the up rows of the same columns.
+//   Wide tile and pair: token rows are the MMA's M operand (128, or 256 over a pair of CTAs), weight rows its
+//   N. A thread owns a token row and the same quarter of the columns out of either half, so that it finds a
+//   gate value and its up value in its own registers; both scales are the same for all its columns of one
+//   weight block, so a value costs half a packed multiply-add.
+//   Few token rows: weight rows are the M (128), 32 token rows the N. A thread owns a weight row and 16
+//   token rows: an eighth of the promotion, 4 KB of token rows to fetch and read instead of 16, and results
+//   that go straight to memory, 32 columns of a row at a time. SwiGLU's up sums cross to the gates' warps
+//   through shared memory. 8-bit results take 256 weight rows, so that a tile has its 128 columns' maximum.
+//   (Token rows as M took 35.5 us for 8 tokens and 49.2 for 64, gate and up; this takes 31.5 and 44.2.)
 //
-// What bounds it. Few rows per expert: the weights' way from HBM (64 tokens, 268 MB of gate and up: 49 us,
-// 5.5 TB/s), and a last round of tiles, 5 us however few they are. Many rows: a block of 256 columns over
-// two CTAs takes 0.43 us where the MMAs alone take 0.27, with shared memory busy for two thirds of it (by its bytes: 64 KB at 128 a clock), and
-// the epilogues are a quarter of a launch of 16 blocks a tile; and, run for seconds, the GPU's power: 8192
-// tokens take 292 us in a burst, 341-350 us at 1.45 GHz and 990 W, of which the promotion's multiply-adds
-// were 67 us. (The library's 8-bit product of the same size, one scale per matrix, no experts, no
-// SwiGLU, takes 246 us at the same power.)
+// What bounds it. Few rows per expert: the weights' way from HBM (64 tokens, 268 MB of gate and up: 44 us,
+// 6.1 TB/s), 3 us before the first ones arrive, and a last round of tiles, 3 to 4 us however few they are.
+// Many rows: a block of 256 columns over two CTAs takes 0.43 us where the MMAs alone take 0.27, with shared
+// memory busy for two thirds of it (by its bytes: 64 KB at 128 a clock), and the epilogues are a quarter
+// of a launch of 16 blocks a tile; and, run for seconds, the GPU's power: 8192 tokens take 292 us in a
+// burst, 341-350 us at 1.45 GHz and 990 W, of which the promotion's multiply-adds were 67 us. (The
+// library's 8-bit product of the same size, one scale per matrix, no experts, no SwiGLU, takes 246 us at
+// the same power.)
 #include <cuda.h>
 #include <cuda_fp8.h>
 
@@ -49,26 +55,40 @@ constexpr int G8_OUT_PITCH = 64 + 16;             // bytes per staged row of res
 constexpr int G8_SLOT = G8_XR + 8;               // floats: the rows' scales, then the weights' two
 constexpr int G8_HELPERS = 4;                    // warps before the promoters: TMA, two for MMA, scales
 constexpr int G8_MOST = 0x7fff0000;              // rows and k: a tile's or a block's end is still a 32-bit number
+constexpr float G8_LOG2E = 1.4426950408889634f, G8_MOST_EXP = 62.f;  // SwiGLU: exp(-g) is kept below 2^62
 constexpr int G8_RING_BYTES = 192 * 1024;
 constexpr int G8_SMEM = G8_RING_BYTES + 1024;    // room to align the ring to 1024
 
-// WR: weight rows per tile. PAIR: two CTAs share a tile (tcgen05 cta_group::2).
-template <int WR, bool PAIR> struct Shape8 {
+// The tiles. WIDE: 128 token rows (the MMA's M) by 256 weight rows (its N). PAIR: 256 by 256 over two CTAs. FEW:
+// 128 weight rows as the MMA's M (with 8-bit results 256, as two MMAs: their columns are a block), by 32
+// token rows as its N.
+enum { G8_FEW = 1, G8_WIDE = 2, G8_PAIR = 3 };
+template <int TILE, bool OUT8> struct Shape8 {
+  static constexpr bool FEW = TILE == G8_FEW, PAIR = TILE == G8_PAIR;
   static constexpr int CTAS = PAIR ? 2 : 1;
-  static constexpr int BM = G8_XR * CTAS;                 // token rows per tile
+  static constexpr int XR = FEW ? G8_XFEW : G8_XR;        // token rows a CTA stages
+  static constexpr int BM = XR * CTAS;                    // token rows per tile
+  static constexpr int WR = FEW && !OUT8 ? 128 : 256;     // weight rows per tile
   static constexpr int WRC = WR / CTAS;                   // weight rows a CTA stages
   static constexpr int WBOX = WR / 2;                     // weight rows per TMA box: a half of the tile
   static constexpr int W_BOXES = WRC / WBOX;              // PAIR: each CTA has one of the halves
-  static constexpr int X_BYTES = G8_XR * G8_BLOCK;
+  static constexpr int X_BYTES = XR * G8_BLOCK;
   static constexpr int STAGE_BYTES = X_BYTES + WRC * G8_BLOCK;
-  static constexpr int STAGES = G8_RING_BYTES / STAGE_BYTES;
-  static constexpr int BUFS = 512 / WR;                   // partial products: all of tensor memory
-  static constexpr int TMEM_COLS = BUFS * WR;
+  // Even, and so is BUFS: a stage and a partial product are always the same MMA warp's. With an odd number
+  // the two warps would take a stage's uses in turn, and the one that is ahead would find the phase it
+  // waits for in the one before it, whose parity is the other's: a use of data not yet there.
+  static constexpr int STAGES = G8_RING_BYTES / STAGE_BYTES / 2 * 2;
+  static constexpr int MMAS = FEW ? WR / 128 : 1;         // per 32 k
+  static constexpr int PART = FEW ? MMAS * XR : WR;       // columns of tensor memory of a partial product
+  static constexpr int BUFS = FEW ? 4 : 2;                // partial products
+  static_assert(STAGES % 2 == 0 && BUFS % 2 == 0, "two MMA warps");
+  static constexpr int TMEM_COLS = BUFS * PART;
   static constexpr int PROMOTERS = 8;                     // warps
   static constexpr int THREADS = (G8_HELPERS + PROMOTERS) * 32;
-  static constexpr int COLS = WR / 4;                     // columns a promoter thread has of either half
+  static constexpr int COLS = WR / 4;                     // columns a promoter thread has of either half (FEW: one)
+  static constexpr int TOKENS = XR / 2;                   // FEW: token rows a promoter thread has
   // 128 accumulators: the helpers hand some of their registers to the promoters (88 / 208: 1-3 % slower)
-  static constexpr bool SPLIT_REGS = COLS > 32;
+  static constexpr bool SPLIT_REGS = !FEW;
 };
 constexpr int G8_REGS_LAUNCH = 168, G8_REGS_FEW = 72, G8_REGS_MANY = 216;
 static_assert(G8_HELPERS * G8_REGS_FEW + 8 * G8_REGS_MANY <= (G8_HELPERS + 8) * G8_REGS_LAUNCH, "register split");
@@ -125,22 +145,25 @@ __device__ __forceinline__ void tmem_get_32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
-// 32 columns from either address.
-__device__ __forceinline__ void tmem_get_32_32(uint32_t a, uint32_t b, uint32_t (&r)[64]) {
+__device__ __forceinline__ void tmem_get_16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%64];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64 + 16];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47}, [%65];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65 + 16];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+// 16 columns from either address.
+__device__ __forceinline__ void tmem_get_16_16(uint32_t a, uint32_t b, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(a), "r"(b)
       : "memory");
 }
@@ -245,7 +268,7 @@ __device__ __forceinline__ Tile8 locate_tile8(int t, int& cursor, int E, const i
 // the same with PACKED products or single ones: 16-bit results are 1-2 % faster with the packed (65,536
 // rows 257 -> 253 us), 8-bit results with the single ones (257, packed 260).
 template <bool PACKED, int N> __device__ __forceinline__ void swiglu_pairs(const uint64_t (&gate)[N], uint64_t (&up)[N]) {
-  constexpr float LOG2E = 1.4426950408889634f, MOST = 62.f;
+  constexpr float LOG2E = G8_LOG2E, MOST = G8_MOST_EXP;
   float most = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -267,11 +290,20 @@ template <bool PACKED, int N> __device__ __forceinline__ void swiglu_pairs(const
   }
 }
 
-template <typename T, int WR, bool PAIR, bool SWIGLU>
-__global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(const __grid_constant__ Gemm8Args args) {
-  using S = Shape8<WR, PAIR>;
+// The same for one column per lane, the pair's other one the neighbouring lane's: the same bits.
+__device__ __forceinline__ float swiglu_lane(float g, float u) {
+  const float x = g * -G8_LOG2E, d = 1.f + exp2_approx(fminf(x, G8_MOST_EXP)), pair = __shfl_xor_sync(0xffffffffu, d, 1);
+  const float v = g * (rcp_approx(d * pair) * pair) * u;
+  return x > G8_MOST_EXP ? v * exp2_approx(G8_MOST_EXP - x) : v;
+}
+
+template <typename T, int TILE, bool SWIGLU>
+__global__ void __launch_bounds__(Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::value>::THREADS, 1) gemm8_kernel(const __grid_constant__ Gemm8Args args) {
+  using S = Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::value>;
+  constexpr int WR = S::WR;
+  constexpr bool PAIR = S::PAIR, FEW = S::FEW;
   constexpr bool OUT8 = std::is_same<T, __nv_fp8_e4m3>::value;
-  static_assert(!OUT8 || (SWIGLU && WR == 256), "a tile of SwiGLU columns is one block of 128");
+  static_assert(!OUT8 || SWIGLU, "a tile of SwiGLU columns is one block of 128");
   constexpr int STAGES = S::STAGES, BUFS = S::BUFS;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES];
@@ -281,9 +313,10 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
   __shared__ uint32_t s_tmem;
   __shared__ int s_begin[G8_MAX_E], s_end[G8_MAX_E];
   __shared__ int s_tile_start[G8_MAX_E + 1];
-  __shared__ float s_scale[G8_SLOTS][G8_SLOT];
-  __shared__ float s_top[OUT8 ? 2 : 1][OUT8 ? 2 : 1][G8_XR];  // 8-bit results: largest magnitude of a row in either 64 columns
-  __shared__ __align__(16) unsigned char s_out[S::PROMOTERS][32 * G8_OUT_PITCH];
+  __shared__ __align__(16) float s_scale[G8_SLOTS][G8_SLOT];
+  __shared__ float s_top[OUT8 ? 2 : 1][OUT8 ? 2 : 1][G8_XR];  // 8-bit results: largest magnitude of a row in the warp's columns
+  __shared__ float s_up[FEW && SWIGLU && !OUT8 ? 4 : 1][S::TOKENS * (WR / 2)];  // sums of up rows on their way to the gates' warps
+  __shared__ __align__(16) unsigned char s_out[FEW ? 1 : S::PROMOTERS][32 * G8_OUT_PITCH];
 
   // (uniform to the compiler, so that the roles are too)
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -365,7 +398,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
         // Token rows: one box of 128 where the tile has that many, else boxes of 32 as far as there are rows.
         // What is multiplied in the others' place is never read.
-        auto rows_of = [&](int c) { return min(max(tile.nvalid - c * G8_XR, 0), G8_XR); };
+        auto rows_of = [&](int c) { return min(max(tile.nvalid - c * S::XR, 0), S::XR); };
         auto boxes_of = [&](int n) { return (n + G8_XFEW - 1) / G8_XFEW; };  // of 32 rows
         const int mine = rows_of(cr), other = PAIR ? rows_of(cr ^ 1) : 0;
         const bool few = mine < G8_XR;
@@ -375,13 +408,13 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         const int b = is_w ? cr + lane : lane - S::W_BOXES;  // half of the weight rows, or box of token rows
         const int colbase = tile.cb * tile_cols;
         const int y = is_w ? (SWIGLU ? (tile.e * 2 + b) * Nout + colbase : tile.e * Nout + colbase + b * S::WBOX)
-                           : tile.row0 + cr * G8_XR + b * G8_XFEW;
+                           : tile.row0 + cr * S::XR + b * G8_XFEW;
         const int off = is_w ? S::X_BYTES + lane * (S::WBOX * G8_BLOCK) : b * (G8_XFEW * G8_BLOCK);
         const void* map = is_w ? static_cast<const void*>(&args.wmap)
                                : few ? static_cast<const void*>(&args.xfew) : static_cast<const void*>(&args.xmap);
         // Weights that no other tile reads make way in L2 first (64 tokens, down 28.0 -> 27.5 us, 82 rows of
-        // 60 experts 21.2 -> 20.5; the narrow tile's SwiGLU stream took 37.6 us with it and 36.0 without)
-        const bool once = WR > 128 && !PAIR && is_w && s_end[tile.e] - s_begin[tile.e] <= S::BM;
+        // 60 experts 21.2 -> 20.5)
+        const bool once = !PAIR && is_w && s_end[tile.e] - s_begin[tile.e] <= S::BM;
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % STAGES, use = it / STAGES;
           int ok = 1;
@@ -417,12 +450,12 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
       // registers), one elected lane issues.
       if (cr == 0) {
         const uint32_t ring_lo = umma_desc_lo(smem_u32(stages));
-        const uint32_t idesc = umma_idesc(0, S::BM, WR);  // format 0 is e4m3 in this kind
+        const uint32_t idesc = FEW ? umma_idesc(0, 128, S::XR) : umma_idesc(0, S::BM, WR);  // format 0 is e4m3 in this kind
         const int n = total_tiles > unit ? ((total_tiles - unit + units - 1) / units) * k_blocks : 0;
         int last = -1;
         for (int it = warp - 1; it < n; it += 2) {
           const int s = it % STAGES, buf = it % BUFS;
-          const uint32_t d = tmem + buf * WR;
+          const uint32_t d = tmem + buf * S::PART;
           if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, wait_ns)) {
             *status = DS_TIMEOUT_FULL;
             break;
@@ -436,6 +469,12 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {  // 32 k = 32 bytes inside the 128-byte rows
+              if (FEW) {
+                umma_f8(d, w_lo + ks * 2, x_lo + ks * 2, UMMA_DESC_HI_K_SW128, idesc, ks != 0);
+                if (S::MMAS == 2)
+                  umma_f8(d + S::XR, w_lo + (128 * G8_BLOCK >> 4) + ks * 2, x_lo + ks * 2, UMMA_DESC_HI_K_SW128, idesc, ks != 0);
+                continue;
+              }
               if (PAIR) umma_f8_pair(d, x_lo + ks * 2, w_lo + ks * 2, UMMA_DESC_HI_K_SW128, idesc, ks != 0);
               else umma_f8(d, x_lo + ks * 2, w_lo + ks * 2, UMMA_DESC_HI_K_SW128, idesc, ks != 0);
             }
@@ -474,8 +513,8 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
       const float *px = nullptr, *pw = nullptr;
       auto enter = [&]() {  // tile t
         const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
-        mine = min(max(tile.nvalid - cr * G8_XR, 0), G8_XR);
-        px = args.xscale + tile.row0 + cr * G8_XR + lane;
+        mine = min(max(tile.nvalid - cr * S::XR, 0), S::XR);
+        px = args.xscale + tile.row0 + cr * S::XR + lane;
         const int col = tile.cb * tile_cols;
         const int nb = SWIGLU ? (lane & 1) * n_blocks + col / G8_BLOCK
                               : min((col + (lane & 1) * (WR / 2)) / G8_BLOCK, n_blocks - 1);
@@ -485,7 +524,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         if (ahead < n) {
           float* slot = s_scale[ahead % G8_SLOTS];
 #pragma unroll
-          for (int r = 0; r < G8_XR; r += 32)
+          for (int r = 0; r < S::XR; r += 32)
             if (r + lane < mine) cp_async_4(slot + r + lane, px + r);
           if (lane < 2) cp_async_4(slot + G8_XR + lane, pw);
           px += args.rows, ++pw;
@@ -512,6 +551,128 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
         if (lane == 0) mbar_arrive(&part_full[buf]);
       }
       cp_async_wait<0>();
+    }
+  } else if constexpr (FEW) {
+    // ---------------------------------------------------------------- promotion and epilogue, few token rows
+    // A thread owns a weight row (8-bit results: a gate row and its up row) and 16 token rows.
+    constexpr int TOK = S::TOKENS, MMAS = S::MMAS;
+    constexpr bool APART = SWIGLU && MMAS == 1;  // warps 0, 1 of a group have the gate rows, 2, 3 the up rows
+    const int q = warp & 3, g = (warp - G8_HELPERS) >> 2;  // quarter of the weight rows; half of the token rows
+    const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + g * TOK;
+    int it = 0, cursor = 0, parity = 0;
+    bool alive = true;
+    for (int t = unit; t < total_tiles; t += units) {
+      const Tile8 tile = locate_tile8<S::BM>(t, cursor, E, s_tile_start, s_begin, s_end);
+      const int rows = tile.nvalid - g * TOK;  // token rows of the warp's
+      uint64_t acc[MMAS][TOK / 2];
+#pragma unroll
+      for (int j = 0; j < TOK / 2; ++j)
+        for (int h = 0; h < MMAS; ++h) acc[h][j] = 0;
+#pragma unroll 1
+      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+        const int buf = it % BUFS;
+        if (alive && !mbar_wait(&part_full[buf], (it / BUFS) & 1, wait_ns)) {
+          *status = DS_TIMEOUT_MMA;
+          alive = false;
+        }
+        __syncwarp();
+        tc_fence_after_sync();
+        const uint32_t from = taddr + buf * S::PART;
+        const float* slot = s_scale[it % G8_SLOTS];
+        uint32_t v[MMAS * TOK];
+        uint64_t sx[TOK / 2];
+        const uint64_t w0 = twice(slot[G8_XR + (APART && q >= 2 ? 1 : 0)]), w1 = twice(slot[G8_XR + 1]);
+        if (rows > 0) {
+          if constexpr (MMAS == 2) tmem_get_16_16(from, from + S::XR, v);
+          else tmem_get_16(from, v);
+#pragma unroll
+          for (int j = 0; j < TOK / 2; j += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(slot + g * TOK + 2 * j);
+            sx[j] = pair64(make_float2(f.x, f.y)), sx[j + 1] = pair64(make_float2(f.z, f.w));
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (elect_one()) mbar_arrive(&part_empty[buf]);
+        __syncwarp();
+        if (rows > 0) {
+#pragma unroll
+          for (int j = 0; j < TOK / 2; ++j) {
+            fma2(acc[0][j], v[2 * j], v[2 * j + 1], mul2(sx[j], w0));
+            if constexpr (MMAS == 2) fma2(acc[1][j], v[TOK + 2 * j], v[TOK + 2 * j + 1], mul2(sx[j], w1));
+          }
+        }
+      }
+      alive = __all_sync(0xffffffffu, alive);
+      if (rows <= 0 || (!alive && !OUT8 && !APART)) continue;
+      const int col = tile.cb * tile_cols + (APART ? q & 1 : q) * 32 + lane;
+      const size_t row0 = tile.row0 + g * TOK;
+      float f[TOK];  // the results. Rows that the tile lacks are worked out too: a branch for each costs more
+#pragma unroll
+      for (int i = 0; i < TOK; ++i) {
+        const float2 v = both(acc[0][i / 2]);
+        f[i] = i & 1 ? v.y : v.x;
+      }
+      if constexpr (APART) {
+        float* up = s_up[parity * 2 + g] + (q & 1) * 32 + lane;  // (two of them: a warp is at most a tile ahead)
+        if (q >= 2) {
+#pragma unroll
+          for (int i = 0; i < TOK; ++i) up[i * (WR / 2)] = f[i];
+        }
+        named_barrier_sync(1 + g, 128);
+        parity ^= 1;
+        if (q >= 2 || !alive) continue;
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) {
+          if (i == TOK / 2 && rows <= TOK / 2) break;
+          f[i] = swiglu_lane(f[i], up[i * (WR / 2)]);
+        }
+      } else if constexpr (SWIGLU) {
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) {
+          if (i == TOK / 2 && rows <= TOK / 2) break;
+          const float2 u = both(acc[MMAS - 1][i / 2]);
+          f[i] = swiglu_lane(f[i], i & 1 ? u.y : u.x);
+        }
+      } else if (args.scale) {
+        const T* sc = static_cast<const T*>(args.scale) + row0;
+        float r[TOK];
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) r[i] = i < rows ? Elem<T>::to_f(sc[i]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) f[i] *= r[i];
+      }
+      T* to = static_cast<T*>(args.C) + row0 * Nout + col;
+      if constexpr (OUT8) {
+        // As in the other tiles; the block's 128 columns are the four warps' lanes. Magnitudes as
+        // integers order like floats, NaN above all.
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) {
+          const uint32_t m = __reduce_max_sync(0xffffffffu, col < Nout ? __float_as_uint(f[i]) & 0x7fffffffu : 0u);
+          if (lane == i) most = m;
+        }
+        uint32_t* tops = reinterpret_cast<uint32_t*>(s_top[parity][g]);  // [warp][token row]
+        if (lane < TOK) tops[q * TOK + lane] = most;
+        named_barrier_sync(1 + g, 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = max(most, tops[i * TOK + lane % TOK]);
+        parity ^= 1;
+        if (!alive) continue;
+        const float top = most > 0x7f800000u ? __int_as_float(0x7fffffff) : fmaxf(__uint_as_float(most), 0x1p-96f);
+        const float inv = 448.f / top;  // of token row `lane`
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) {
+          const float by = __shfl_sync(0xffffffffu, inv, i);
+          if (i < rows && col < Nout)
+            reinterpret_cast<__nv_fp8_storage_t*>(to)[(size_t)i * Nout] = __nv_cvt_float_to_fp8(f[i] * by, __NV_SATFINITE, __NV_E4M3);
+        }
+        if (q == 0 && lane < min(rows, TOK)) args.cscale[(size_t)tile.cb * args.rows + row0 + lane] = top / 448.f;
+      } else {
+#pragma unroll
+        for (int i = 0; i < TOK; ++i)
+          if (i < rows && col < Nout) to[(size_t)i * Nout] = Elem<T>::from_f(f[i]);
+      }
     }
   } else {
     // ---------------------------------------------------------------- promotion and epilogue
@@ -557,13 +718,12 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
           const float* slot = s_scale[it % G8_SLOTS];
           const float sx = slot[q * 32 + lane];
           const uint64_t f0 = twice(sx * slot[G8_XR]), f1 = twice(sx * slot[G8_XR + 1]);
-          // as many columns at once as there are registers for: a load takes its 70 clocks either way
-          constexpr int AT_ONCE = S::COLS > 32 ? 32 : 64, GROUPS = 2 * S::COLS / AT_ONCE;
+          // as many columns at once as there are registers for
+          constexpr int AT_ONCE = 32, GROUPS = 2 * S::COLS / AT_ONCE;
 #pragma unroll
           for (int c = 0; c < GROUPS; ++c) {
             uint32_t v[AT_ONCE];
-            if constexpr (AT_ONCE == 64) tmem_get_32_32(from, from + WR / 2, v);
-            else tmem_get_32(from + (c * 32 / S::COLS) * (WR / 2) + c * 32 % S::COLS, v);
+            tmem_get_32(from + (c * 32 / S::COLS) * (WR / 2) + c * 32 % S::COLS, v);
             if (c + 1 == GROUPS) close();
 #pragma unroll
             for (int j = 0; j < AT_ONCE / 2; ++j) {
@@ -677,7 +837,7 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
           }
           store64(c, o);
         }
-      } else if constexpr (S::COLS == 64) {
+      } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t o[32];
@@ -687,17 +847,6 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
             o[j] = pack16<T>(v.x * row_scale, v.y * row_scale);
           }
           store128(h * (WR / 2), o);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 2 * S::COLS; c += 32) {
-          uint32_t o[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 v = both(acc[c / S::COLS][c % S::COLS / 2 + j]);
-            o[j] = pack16<T>(v.x * row_scale, v.y * row_scale);
-          }
-          store64(c < S::COLS ? c : WR / 2 + c - S::COLS, o);
         }
       }
     }
@@ -715,25 +864,25 @@ __global__ void __launch_bounds__(Shape8<WR, PAIR>::THREADS, 1) gemm8_kernel(con
 
 // ---- host side ------------------------------------------------------------------------------
 // How many blocks (pairs: clusters of two) fit the device at once; asked once per kernel and device.
-template <typename T, int WR, bool PAIR, bool SWIGLU> static int units8(int sms, int* out) {
+template <typename T, int TILE, bool SWIGLU> static int units8(int sms, int* out) {
   static std::atomic<int> cached[MAX_DEVICES];
   int dev = 0;
   SY_CUDA(cudaGetDevice(&dev));
   int units = cached[dev].load(std::memory_order_acquire);
   if (!units) {
-    auto kern = gemm8_kernel<T, WR, PAIR, SWIGLU>;
+    auto kern = gemm8_kernel<T, TILE, SWIGLU>;
     SY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G8_SMEM));
-    if (Shape8<WR, PAIR>::SPLIT_REGS) {
+    if (Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::value>::SPLIT_REGS) {
       // the promoters' register request waits for ever if the block was launched with fewer
       cudaFuncAttributes attr;
       SY_CUDA(cudaFuncGetAttributes(&attr, kern));
       if (attr.numRegs < G8_REGS_LAUNCH)
         return fail(SY_ERR_CUDA, "grouped_gemm_fp8: built with %d registers per thread, needs %d", attr.numRegs, G8_REGS_LAUNCH);
     }
-    if (PAIR) {
+    if (Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::value>::PAIR) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(sms & ~1);
-      cfg.blockDim = dim3(Shape8<WR, PAIR>::THREADS);
+      cfg.blockDim = dim3(Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::value>::THREADS);
       cfg.dynamicSmemBytes = G8_SMEM;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -746,7 +895,7 @@ template <typename T, int WR, bool PAIR, bool SWIGLU> static int units8(int sms,
       if (units > sms / 2) units = sms / 2;
     } else {
       int per_sm = 0;
-      SY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, Shape8<WR, PAIR>::THREADS, G8_SMEM));
+      SY_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::value>::THREADS, G8_SMEM));
       units = per_sm >= 1 ? sms : 0;
     }
     if (units < 1) return fail(SY_ERR_CUDA, "grouped_gemm_fp8: no block of the kernel fits on this device");
@@ -756,13 +905,13 @@ template <typename T, int WR, bool PAIR, bool SWIGLU> static int units8(int sms,
   return SY_OK;
 }
 
-template <typename T, int WR, bool PAIR, bool SWIGLU>
+template <typename T, int TILE, bool SWIGLU>
 static int launch8(Gemm8Args a, const void* x, const void* w, cudaStream_t stream) {
-  using S = Shape8<WR, PAIR>;
+  using S = Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::value>;
   int sms = 0, units = 0;
   int rc = device_sm_count(&sms);
   if (rc != SY_OK) return rc;
-  rc = units8<T, WR, PAIR, SWIGLU>(sms, &units);
+  rc = units8<T, TILE, SWIGLU>(sms, &units);
   if (rc != SY_OK) return rc;
   const uint64_t w_rows = (uint64_t)a.experts * (SWIGLU ? 2 : 1) * a.Nout;
   rc = tensor_map_2d(&a.wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, w_rows, (uint64_t)a.K, S::WBOX, G8_BLOCK);
@@ -771,37 +920,33 @@ static int launch8(Gemm8Args a, const void* x, const void* w, cudaStream_t strea
   if (rc != SY_OK) return rc;
   rc = tensor_map_2d(&a.xfew, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XFEW, G8_BLOCK);
   if (rc != SY_OK) return rc;
-  auto kern = gemm8_kernel<T, WR, PAIR, SWIGLU>;
-  if (PAIR) return launch_cluster_kernel(kern, 2, 2 * units, S::THREADS, G8_SMEM, stream, "grouped_gemm_fp8 launch", a);
+  auto kern = gemm8_kernel<T, TILE, SWIGLU>;
+  if (S::PAIR) return launch_cluster_kernel(kern, 2, 2 * units, S::THREADS, G8_SMEM, stream, "grouped_gemm_fp8 launch", a);
   return launch_kernel(kern, units, S::THREADS, G8_SMEM, stream, "grouped_gemm_fp8 launch", a);
 }
 
 template <typename T, bool SWIGLU>
 static int dispatch8(const Gemm8Args& a, int tile, const void* x, const void* w, cudaStream_t s) {
-  if constexpr (!std::is_same<T, __nv_fp8_e4m3>::value)
-    if (tile == 1) return launch8<T, 128, false, SWIGLU>(a, x, w, s);
-  return tile == 2 ? launch8<T, 256, false, SWIGLU>(a, x, w, s) : launch8<T, 256, true, SWIGLU>(a, x, w, s);
+  return tile == G8_FEW    ? launch8<T, G8_FEW, SWIGLU>(a, x, w, s)
+         : tile == G8_WIDE ? launch8<T, G8_WIDE, SWIGLU>(a, x, w, s)
+                           : launch8<T, G8_PAIR, SWIGLU>(a, x, w, s);
 }
 
 // Which tile a batch gets; the bits are the same. Measured on a B200 with the benchmark's layer (64 experts,
-// gate and up 2048 x 2048 with SwiGLU, down 2048 x 1024), us for the narrow / wide / pair tile:
-//   1 token     gate-up 11.0 / 14.4 / 14.2    down  6.9 /  8.2 /  9.6   (wide: fewer tiles than SMs)
-//   8 tokens            37.0 / 37.1 / 45.5         21.6 / 21.0 / 28.6
-//   16 tokens           43.2 / 42.3
-//   64 tokens           51.2 / 50.0 / 64.7         29.4 / 26.7 / 37.6   (gate-up on another card 48.0 / 49.9;
-//                       31.4 / 28.9 with half the k, 29.9 / 27.6 with half the columns)
-//   512 tokens          53.9 / 50.7 / 67.6         31.0 / 26.9 / 39.3   (64 rows per expert)
-//   1024 tokens         75.8 / 67.4 / 72.4         45.0 / 39.2 / 43.8
-//   4096 tokens          204 /  167 /  168          118 /  100 /  102
-//   8192 tokens          372 /  305 /  303          219 /  184 /  183   (1024 rows per expert)
-// So: pairs from 768 rows per expert; the wide tile where it gives every SM a tile, SwiGLU only beyond a
-// row per expert; else the narrow one, which has twice the tiles.
-static int choose_tile8(int rows, int experts, int n_out, bool swiglu, int sms) {
-  if (rows >= 768LL * experts) return 3;
-  if (rows > 64LL * experts) return 2;
-  const long long cols = swiglu ? 128 : 256;
-  const long long wide = (long long)(rows < experts ? rows : experts) * ((n_out + cols - 1) / cols);
-  return wide >= sms && (!swiglu || rows > experts) ? 2 : 1;
+// gate and up 2048 x 2048 with SwiGLU, down 2048 x 1024), us for the few / wide / pair tile:
+//   1 token     gate-up  9.6 / 13.5 / 14.2    down  6.9 /  8.6 /  9.6    8-bit results 11.8 / 14.3
+//   8 tokens            31.6 / 36.7 / 45.5         18.4 / 21.0 / 28.6                  33.7 / 38.1
+//   64 tokens           44.2 / 50.3 / 64.7         26.0 / 26.8 / 37.6                  47.7 / 51.5
+//   160 tokens          46.6 / 50.1                26.5 / 27.3                         47.1 / 50.9   (20 rows per expert)
+//   192 tokens          50.2 / 49.7                27.9 / 27.3                         47.6 / 50.9
+//   256 tokens          61.1 / 49.8                34.9 / 27.4                         52.2 / 50.7
+//   512 tokens           106 / 50.7 / 67.6         58.5 / 26.9 / 39.3
+//   1024 tokens                67.4 / 72.4                39.2 / 43.8
+//   4096 tokens                 167 /  168                 100 /  102
+//   8192 tokens                 305 /  303                 184 /  183   (1024 rows per expert)
+// So: few up to 20 rows per expert (its 32 token rows are then seldom too few), pairs from 768, else wide.
+static int choose_tile8(int rows, int experts) {
+  return rows <= 20LL * experts ? G8_FEW : rows < 768LL * experts ? G8_WIDE : G8_PAIR;
 }
 
 }  // namespace sy
@@ -818,8 +963,8 @@ extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const vo
   SY_REQUIRE(n_out > 0 && n_out % 8 == 0, "grouped_gemm_fp8: n_out must be a multiple of 8 (got %d)", n_out);
   SY_REQUIRE(!(swiglu && scale), "grouped_gemm_fp8: swiglu and scale are separate epilogues");
   SY_REQUIRE(c_scale || dtype == SY_DTYPE_F16 || dtype == SY_DTYPE_BF16, "grouped_gemm_fp8: dtype must be f16 or bf16");
-  SY_REQUIRE(!c_scale || (swiglu && n_out % 16 == 0 && tile != 1),
-             "grouped_gemm_fp8: 8-bit results are SwiGLU's, of a multiple of 16 columns, from the wide tiles");
+  SY_REQUIRE(!c_scale || (swiglu && n_out % 16 == 0),
+             "grouped_gemm_fp8: 8-bit results are SwiGLU's, of a multiple of 16 columns");
   SY_REQUIRE(tile >= 0 && tile <= 3, "grouped_gemm_fp8: tile 0..3 (got %d)", tile);
   SY_REQUIRE((int64_t)n_experts * 2 * n_out <= 0x7fffff00, "grouped_gemm_fp8: more than 2^31 weight rows");
   if (rows == 0) return SY_OK;
@@ -841,13 +986,7 @@ extern "C" int sy_grouped_gemm_fp8(const void* x, const float* x_scale, const vo
   a.status = device_status_word();
   if (!a.status) return SY_ERR_CUDA;
   a.wait_ns = wait_limit_ns();
-  if (tile == 0) {
-    int sms = 0;
-    const int rc = device_sm_count(&sms);
-    if (rc != SY_OK) return rc;
-    tile = choose_tile8(rows, n_experts, n_out, swiglu != 0, sms);
-    if (c_scale && tile == 1) tile = 2;
-  }
+  if (tile == 0) tile = choose_tile8(rows, n_experts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c_scale) return dispatch8<__nv_fp8_e4m3, true>(a, tile, x, w, s);
   if (dtype == SY_DTYPE_F16) return swiglu ? dispatch8<__half, true>(a, tile, x, w, s) : dispatch8<__half, false>(a, tile, x, w, s);

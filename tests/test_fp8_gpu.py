@@ -113,7 +113,8 @@ def operands(counts, K, N, swiglu, seed):
 
 
 SHAPES = [([1], 16, 8), ([3, 0, 1, 70], 128, 128), ([0, 0, 5], 144, 136), ([130, 1, 257], 272, 392), ([64] * 8, 256, 256),
-          ([0, 300, 0, 33, 1, 0], 1040, 1000), ([1] * 40, 2048, 64), ([600, 200], 512, 264)]
+          ([0, 300, 0, 33, 1, 0], 1040, 1000), ([1] * 40, 2048, 64), ([600, 200], 512, 264),
+          ([33, 5, 64, 1] * 8, 656, 1040)]  # the last: several rounds of every tile
 
 
 @pytest.mark.parametrize("counts,K,N", SHAPES)
@@ -169,7 +170,7 @@ def test_swiglu_straight_to_8_bits(Q, counts, K, N):
         assert ((s * 448 - m.clamp(min=2.0 ** -96)).abs() <= d.amax(1) + 2.0 ** -22 * m).all()
         far = d + (v.abs() + d) * (2.0 ** -4 + 2.0 ** -21) + 2.0 ** -10 * s[:, None]
         assert ((c * s[:, None] - v).abs() <= far).all()
-    for tile in (2, 3):
+    for tile in (1, 2, 3):
         again = kernels.ext().grouped_gemm_fp8(*dev, True, None, torch.float8_e4m3fn, tile)
         assert torch.equal(again[0].view(torch.uint8), got.q.view(torch.uint8))
         assert torch.equal(again[1].view(torch.int32), got.scale.view(torch.int32))
