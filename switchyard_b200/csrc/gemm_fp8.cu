@@ -259,6 +259,11 @@ __device__ __forceinline__ Tile8 locate_tile8(int t, int& cursor, int E, const i
   return tile;
 }
 
+// The exponent (to base 2) of what is left of exp(g) once 2^-62 is taken out, for gates below -43. Two
+// roundings, written out: as one multiply-add the exponent is off by another 2^-18, and a row would
+// have other bits in the tile whose form the compiler happens to contract.
+__device__ __forceinline__ float swiglu_rest(float g) { return __fsub_rn(G8_MOST_EXP, __fmul_rn(g, -G8_LOG2E)); }
+
 // up <- silu(gate) * up for N pairs of columns. The reciprocals of a pair's 1 + exp(-g) come from the one
 // of their product (the special-function unit is what an epilogue waits for). exp and the
 // reciprocal are the approximate ones, exp within 2^-22 and the rounding of its argument (2^-18 at
@@ -273,7 +278,7 @@ template <bool PACKED, int N> __device__ __forceinline__ void swiglu_pairs(const
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const float2 g = both(gate[j]), u = both(up[j]);
-    const float2 x = PACKED ? both(mul2(gate[j], twice(-LOG2E))) : make_float2(g.x * -LOG2E, g.y * -LOG2E);
+    const float2 x = PACKED ? both(mul2(gate[j], twice(-LOG2E))) : make_float2(__fmul_rn(g.x, -LOG2E), __fmul_rn(g.y, -LOG2E));
     const float x0 = x.x, x1 = x.y;
     const float d0 = 1.f + exp2_approx(fminf(x0, MOST)), d1 = 1.f + exp2_approx(fminf(x1, MOST));
     const float r = rcp_approx(d0 * d1);
@@ -285,16 +290,16 @@ template <bool PACKED, int N> __device__ __forceinline__ void swiglu_pairs(const
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float2 g = both(gate[j]), v = both(up[j]);
-      up[j] = pair64(make_float2(v.x * exp2_approx(fminf(MOST - g.x * -LOG2E, 0.f)), v.y * exp2_approx(fminf(MOST - g.y * -LOG2E, 0.f))));
+      up[j] = pair64(make_float2(v.x * exp2_approx(fminf(swiglu_rest(g.x), 0.f)), v.y * exp2_approx(fminf(swiglu_rest(g.y), 0.f))));
     }
   }
 }
 
 // The same for one column per lane, the pair's other one the neighbouring lane's: the same bits.
 __device__ __forceinline__ float swiglu_lane(float g, float u) {
-  const float x = g * -G8_LOG2E, d = 1.f + exp2_approx(fminf(x, G8_MOST_EXP)), pair = __shfl_xor_sync(0xffffffffu, d, 1);
+  const float x = __fmul_rn(g, -G8_LOG2E), d = 1.f + exp2_approx(fminf(x, G8_MOST_EXP)), pair = __shfl_xor_sync(0xffffffffu, d, 1);
   const float v = g * (rcp_approx(d * pair) * pair) * u;
-  return x > G8_MOST_EXP ? v * exp2_approx(G8_MOST_EXP - x) : v;
+  return x > G8_MOST_EXP ? v * exp2_approx(swiglu_rest(g)) : v;
 }
 
 template <typename T, int TILE, bool SWIGLU>

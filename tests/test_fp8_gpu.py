@@ -226,6 +226,51 @@ def test_swiglu_of_very_negative_gates(Q, dtype):
             assert got.shape == (M, n) and ((got - v).abs() <= e).all(), ((got - v).abs() / e).max()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, torch.float8_e4m3fn])
+def test_swiglu_of_very_negative_gates_in_every_tile(Q, dtype):
+    """As above, through each tile, with more rows than one CTA of a pair has, two column blocks and an expert
+    whose gates are all below -43. One term per sum, its operands of 4, 4 and 8 significant bits and powers of
+    two: gate and value are exact, the bound is the one above, and the bits are the same in every tile."""
+    from switchyard_b200 import kernels
+    counts, N, K = [300, 70], 144, 16
+    M, E = sum(counts), len(counts)
+    g = torch.Generator().manual_seed(31)
+    xq, wq = torch.zeros(M, K), torch.zeros(E, 2 * N, K)
+    xq[:, 0] = 0.8 + 0.2 * torch.rand(M, generator=g)
+    wq[0, :N, 0] = -(56 + 34 * torch.rand(N, generator=g))
+    wq[1, :N, 0] = 150 * torch.rand(N, generator=g) - 130
+    wq[:, N:, 0] = torch.randn(E, N, generator=g) * 3
+    xq, wq = xq.to(torch.float8_e4m3fn), wq.to(torch.float8_e4m3fn)
+    xs = (torch.randint(256, 320, (1, M), generator=g) / 256.0)
+    up = torch.tensor([2.0 ** 60, 2.0 ** -4] if dtype is HF else [2.0 ** 40, 2.0 ** 40])
+    ws = torch.ones(E, 4, 1)
+    ws[:, 2:, 0] = up[:, None]
+    offsets = torch.tensor([0] + counts).cumsum(0).int()
+    e = torch.repeat_interleave(torch.arange(E), torch.tensor(counts))
+    x = xq.double()[:, :1] * xs.double().t()
+    gate, value = x * wq.double()[e, :N, 0], x * wq.double()[e, N:, 0] * up.double()[e, None]
+    assert (gate[:300] < -43).all() and (gate[300:] > -43).any() and (gate[300:] < -43).any()
+    ref = torch.where(gate > 0, gate / (1 + torch.exp(-gate)), gate * torch.exp(gate) / (1 + torch.exp(gate))) * value
+    d = 2.0 ** -16 * ref.abs() + (gate * value).abs() * 2.0 ** -126
+    dev = [t.to(DEV) for t in (xq, xs, wq, ws, offsets)]
+    first = None
+    for tile in (1, 2, 3):
+        got = kernels.ext().grouped_gemm_fp8(*dev, True, None, dtype, tile)
+        if dtype is torch.float8_e4m3fn:
+            bits = (got[0].view(torch.uint8), got[1].view(torch.int32))
+            for b, cols in enumerate((slice(0, 128), slice(128, N))):
+                v, off, s = ref[:, cols], d[:, cols], got[1].cpu().double()[b]
+                m = v.abs().amax(1)
+                assert ((s * 448 - m.clamp(min=2.0 ** -96)).abs() <= off.amax(1) + 2.0 ** -22 * m).all(), tile
+                far = off + (v.abs() + off) * (2.0 ** -4 + 2.0 ** -21) + 2.0 ** -10 * s[:, None]
+                assert ((got[0].cpu().double()[:, cols] * s[:, None] - v).abs() <= far).all(), tile
+        else:
+            bits = (got.view(torch.int16),)
+            assert ((got.cpu().double() - ref).abs() <= d + rounding(ref.abs() + d, dtype)).all(), tile
+        first = first or bits
+        assert all(torch.equal(a, b) for a, b in zip(bits, first)), tile
+
+
 def test_a_rows_bits_do_not_depend_on_its_expert_s_other_rows(Q):
     from switchyard_b200 import kernels
     offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([200], 384, 160, False, 3))
