@@ -8,7 +8,7 @@ multiplies. Beyond the reference, which has 16-bit experts only.
     out = kernels.moe_layer(h, router, gate_up8, down8, top_k, norm)
 
 For inference: no call here has a gradient, and an input that requires one is refused while
-gradients are recorded. Everything is enqueued on the current stream; nothing synchronises, there are
+gradients are recorded, one with a forward-mode tangent always. Everything is enqueued on the current stream; nothing synchronises, there are
 no workspaces. Make the first call on a device outside a capture (it loads the library there)."""
 
 from typing import NamedTuple
@@ -60,6 +60,7 @@ def refuse(name, *weights):
 def _no_grad(name, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
+    _rows.refuse_tangents(name, *tensors)
 
 
 def quantize_rows(x, plan=None):

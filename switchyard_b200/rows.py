@@ -10,11 +10,13 @@ csrc/rows.cu. Beyond the reference, which infers only.
 Rows are fp16, bf16 or fp32 with a row of a multiple of 16 bytes, top_k is at most 8. Everything is
 enqueued on the current stream; nothing synchronises. There are no workspaces: what a captured graph
 keeps are the addresses of its tensors. Make the first call on a device outside a capture (it loads
-the library there). RuntimeError on any other argument."""
+the library there). RuntimeError on any other argument, and for an input with a forward-mode
+tangent (the operators have gradients, no forward-mode derivatives)."""
 
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 
@@ -49,6 +51,12 @@ def plan(idx, n_experts):
         idx = idx.clamp(-1, n_experts).to(torch.int32)  # (an id past 32 bits must not come back as another)
     counts, offsets, token, _, pos_of = _ext().sort_by_expert(idx.contiguous(), None, n_experts)
     return SortPlan(counts, offsets, token, pos_of.view(idx.shape))
+
+
+def refuse_tangents(name, *tensors):
+    """Raises for dual tensors: they do not ask for a gradient, so their tangents would get lost in silence."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative: unpack its dual inputs first")
 
 
 def _incoming(d):
@@ -96,6 +104,7 @@ class _Unpermute(torch.autograd.Function):
 def permute_rows(h, plan):
     """x [N*k, H]: row plan.pos_of[t, j] is h[t]. Gradient: every token's rows of dx summed in float32
     in ascending row, rounded once."""
+    refuse_tangents("permute_rows", h)
     h = h.contiguous()
     if torch.is_grad_enabled() and h.requires_grad:
         return _Permute.apply(h, plan.offsets, plan.pos_of)
@@ -106,6 +115,7 @@ def unpermute_rows(y, w, plan):
     """out [N, H]: sum over j of w[t, j] * y[plan.pos_of[t, j]], in float32 in ascending row (the order of
     `combine`), rounded once. w [N, k] in y's dtype or float32, or None for a plain sum. Gradients:
     dy (rows of no choice: zero) and dw, the dot products in float32."""
+    refuse_tangents("unpermute_rows", y, w)
     y = y.contiguous()
     w = w.contiguous() if w is not None else None
     if torch.is_grad_enabled() and (y.requires_grad or (w is not None and w.requires_grad)):

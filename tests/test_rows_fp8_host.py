@@ -114,6 +114,33 @@ def test_8_bit_calls_refuse_inputs_that_require_a_gradient(lib):
             call(t(4, 32, grad=True))
 
 
+def test_forward_mode_tangents_are_refused(lib):
+    """A dual tensor asks for no gradient: a call that looked at that alone would drop its tangent."""
+    from torch.autograd import forward_ad as fwd
+
+    from switchyard_b200 import fp8, rows
+    pos = torch.zeros(4, 2, dtype=torch.int32)
+    plan = rows.SortPlan(torch.zeros(8, dtype=torch.int32), torch.zeros(9, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), pos)
+    h, y, w = torch.zeros(4, 128), torch.zeros(8, 128), torch.zeros(4, 2)
+    x8, w8 = fp8.Rows8(h.to(torch.float8_e4m3fn), torch.zeros(1, 4)), fp8.Weight8(torch.zeros(1, 8, 128).to(torch.float8_e4m3fn), torch.zeros(1, 1, 1))
+    offsets = torch.zeros(2, dtype=torch.int32)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        calls = (lambda: rows.permute_rows(dual(h), plan), lambda: rows.permute_rows(dual(h)[:, ::2], plan),
+                 lambda: rows.unpermute_rows(dual(y), w, plan), lambda: rows.unpermute_rows(y, dual(w), plan),
+                 lambda: rows.unpermute_rows(dual(y), None, plan), lambda: fp8.quantize_rows(dual(h)),
+                 lambda: fp8.quantize_weight(dual(torch.zeros(1, 8, 128))),
+                 lambda: fp8.grouped_gemm(x8._replace(scale=dual(x8.scale)), w8, offsets),
+                 lambda: fp8.grouped_gemm(x8, w8, offsets, scale=dual(torch.zeros(4))))
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="CUDA"):  # no tangent: the next check
+            rows.permute_rows(h, plan)
+
+
 def test_the_plain_quantiser_is_torchs_e4m3(lib):
     """nearest8 against torch's own conversion on every 16-bit value it can take, ties included."""
     v = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(torch.float16).float()
