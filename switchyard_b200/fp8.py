@@ -29,12 +29,28 @@ class Rows8(NamedTuple):
         return (self.q.float() * self.scale.t().repeat_interleave(128, 1)[:, :K]).to(dtype)
 
 
-class Weight8(NamedTuple):
-    """q float8_e4m3fn [E, N, K], scale float32 [E, halves * ceil(N/halves/128), ceil(K/128)] for blocks
-    of 128 x 128; a gate_up stack counts its blocks in each half on its own (halves 2), which
-    is the plain layout when the halves are multiples of 128."""
+class _Weight8(NamedTuple):
     q: torch.Tensor
     scale: torch.Tensor
+
+
+class Weight8(_Weight8):
+    """q float8_e4m3fn [E, N, K], scale float32 [E, halves * ceil(N/halves/128), ceil(K/128)] for blocks
+    of 128 x 128; a gate_up stack counts its blocks in each half on its own (halves 2), which
+    is the plain layout when the halves are multiples of 128. Where they are not, the two layouts can have
+    the same shape (N = 400: four blocks of rows either way), so a weight says which it has: `halves`, None
+    in one put together from its two tensors alone, which is taken for what it is used as."""
+
+    halves = None
+
+    def __new__(cls, q, scale, halves=None):
+        self = super().__new__(cls, q, scale)
+        if halves is not None:
+            self.halves = halves
+        return self
+
+    def _replace(self, **changed):
+        return type(self)(**{**self._asdict(), "halves": self.halves, **changed})
 
     @property
     def shape(self):
@@ -44,8 +60,19 @@ class Weight8(NamedTuple):
     def device(self):
         return self.q.device
 
-    def dequantize(self, dtype=torch.float32, halves=1):
+    def check_halves(self, name, halves):
+        """Raises where the blocks of rows are known to be counted otherwise than in `halves`."""
+        if self.halves not in (None, halves) and self.q.shape[1] % 256:
+            raise RuntimeError(f"{name}: a weight of {self.q.shape[1]} rows quantised with halves={self.halves} has other "
+                               f"blocks than halves={halves}")
+
+    def dequantize(self, dtype=torch.float32, halves=None):
+        """The values, [E, N, K]. halves: needed where the weight does not know its own."""
         E, N, K = self.q.shape
+        halves = halves or self.halves or 1
+        self.check_halves("dequantize", halves)
+        if self.scale.shape[1] != halves * ((N // halves + 127) // 128):
+            raise RuntimeError(f"dequantize: {self.scale.shape[1]} blocks of rows are not those of {N} rows with halves={halves}")
         s = self.scale.reshape(E * halves, -1, self.scale.shape[-1])
         s = s.repeat_interleave(128, 1)[:, :N // halves].repeat_interleave(128, 2)[:, :, :K]
         return (self.q.float() * s.reshape(E, N, K)).to(dtype)
@@ -78,7 +105,7 @@ def quantize_rows(x, plan=None):
 def quantize_weight(w, halves=1):
     """Weight8 of w [E, N, K] (fp16, bf16 or fp32, K a multiple of 16). halves=2 for a gate_up stack."""
     _no_grad("quantize_weight", w)
-    return Weight8(*_rows._ext().quantize_weight(w.contiguous(), halves))
+    return Weight8(*_rows._ext().quantize_weight(w.contiguous(), halves), halves)
 
 
 def grouped_gemm(x, w, offsets, swiglu=False, scale=None, dtype=torch.bfloat16):
@@ -89,6 +116,7 @@ def grouped_gemm(x, w, offsets, swiglu=False, scale=None, dtype=torch.bfloat16):
     where it is computed (scale = m / 448 and q = e4m3(v * (448 / m)) of the float32 values). Rows of no
     expert are zero. A row's bits depend on nothing but the row and its expert's weights."""
     _no_grad("grouped_gemm", x.q, x.scale, w.q, w.scale, scale)
+    w.check_halves("grouped_gemm", 2 if swiglu else 1)
     out = _rows._ext().grouped_gemm_fp8(x.q, x.scale, w.q, w.scale, offsets, swiglu, scale, dtype)
     return Rows8(*out) if dtype is torch.float8_e4m3fn else out
 

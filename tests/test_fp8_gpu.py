@@ -396,6 +396,26 @@ def test_the_decoder_on_8_bit_experts(Q):
     assert d8.generate(prompts, 8, graph=True) == d8.generate(prompts, 8, graph=False)
 
 
+def test_a_stack_quantised_as_one_is_not_taken_for_gate_and_up(Q):
+    """Experts of width 200: the two layouts' scales have the same shape (four blocks of rows)."""
+    from switchyard_b200 import kernels
+    h, router, gate_up, _ = layer(4, 8, 2, 128, 200, BF)
+    plain, halved = Q.quantize_weight(gate_up), Q.quantize_weight(gate_up, halves=2)
+    assert plain.scale.shape == halved.scale.shape and not torch.equal(plain.scale, halved.scale)
+    x8, offsets = Q.quantize_rows(h), torch.tensor([0] + [4] * 8, dtype=torch.int32, device=DEV)
+    for w, swiglu in ((plain, True), (halved, False)):
+        with pytest.raises(RuntimeError, match="halves"):
+            Q.grouped_gemm(x8, w, offsets, swiglu=swiglu)
+    down = Q.quantize_weight(torch.zeros(8, 128, 208, device=DEV))
+    with pytest.raises(RuntimeError, match="halves"):
+        kernels.moe_layer(h, router, plain, down, 2, False)
+    x, wide = x8.dequantize().cpu().double(), plain.dequantize()[0].cpu().double()
+    want, mag = x @ wide.t(), x.abs() @ wide.abs().t()
+    got = Q.grouped_gemm(x8, plain, offsets).cpu().double()
+    # (dequantize rounds value times scale to float32 on either side)
+    assert ((got - want).abs() <= product_bound(want, mag, 128, BF)[1] + 2.0 ** -22 * mag).all()
+
+
 def test_streams_and_graphs(Q):
     """The same call on two streams at once and replayed from a graph, on new inputs."""
     offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([20, 0, 300], 256, 256, True, 9))

@@ -172,6 +172,43 @@ def test_dequantize_is_the_layout(lib):
     assert ((w8.dequantize(halves=2) - w).abs() <= w.abs() * (2.0 ** -4 + 2.0 ** -22) + 2.0 ** -10 * 6 / 448).all()
 
 
+def test_a_weight_knows_how_its_blocks_are_counted(lib):
+    """400 rows are four blocks of rows either way: 128, 128, 128, 16, or 128, 72 in each half. The layout that
+    was not asked for has to be refused, not read with the wrong scales."""
+    import copy
+
+    from switchyard_b200 import fp8
+    g = torch.Generator().manual_seed(2)
+    w = torch.randn(1, 400, 128, generator=g)
+    q, s = zip(*[rc.quantize64(p, 128) for p in w.view(2, 200, 128)])
+    w8 = fp8.Weight8(torch.cat(q).view(1, 400, 128).float().to(torch.float8_e4m3fn), torch.cat(s).view(1, 4, 1), halves=2)
+    q, scale = w8
+    assert len(w8) == 2 and q is w8.q and scale is w8.scale
+    near = lambda v: ((v - w).abs() <= w.abs() * (2.0 ** -4 + 2.0 ** -22) + 2.0 ** -10 * 6 / 448).all()
+    for kept in (w8, copy.deepcopy(w8), w8._replace(q=w8.q.clone())):
+        assert kept.halves == 2 and near(kept.dequantize()) and near(kept.dequantize(halves=2))
+        with pytest.raises(RuntimeError, match="halves"):
+            kept.dequantize(halves=1)
+    bare = fp8.Weight8(w8.q, w8.scale)
+    assert bare.halves is None and near(bare.dequantize(halves=2))
+    x8, offsets = fp8.Rows8(torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(1, 4)), torch.zeros(2, dtype=torch.int32)
+    plain = fp8.Weight8(w8.q, w8.scale, halves=1)
+    with pytest.raises(RuntimeError, match="halves"):
+        fp8.grouped_gemm(x8, plain, offsets, swiglu=True)
+    with pytest.raises(RuntimeError, match="halves"):
+        fp8.grouped_gemm(x8, w8, offsets)
+    for weight, swiglu in ((w8, True), (plain, False), (bare, True), (bare, False)):
+        with pytest.raises(RuntimeError, match="CUDA"):  # the next check
+            fp8.grouped_gemm(x8, weight, offsets, swiglu=swiglu)
+    # halves that are multiples of 128: one layout
+    even = fp8.Weight8(torch.zeros(1, 256, 128).to(torch.float8_e4m3fn), torch.zeros(1, 2, 1), halves=1)
+    even.dequantize(halves=2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fp8.grouped_gemm(x8, even, offsets, swiglu=True)
+    with pytest.raises(RuntimeError, match="blocks of rows"):  # three blocks where two halves of 136 have four
+        fp8.Weight8(torch.zeros(1, 272, 128).to(torch.float8_e4m3fn), torch.zeros(1, 3, 1)).dequantize(halves=2)
+
+
 def test_expert_parallelism_refuses_8_bit_experts(lib):
     from switchyard_b200 import fp8
     from switchyard_b200.ep import ExpertParallel
