@@ -264,8 +264,8 @@ int sy_unpermute_rows_grad(const void* dout, const void* y, const void* w, int w
 /* ---- experts in 8-bit floats --------------------------------------------------------------------
  * No counterpart in the reference. e4m3 values with a float32 scale for each block: 1 x 128 for
  * rows, 128 x 128 for weights. With m = max(largest magnitude of the block, 2^-96):
- * scale = m / 448, q = e4m3(448 x / m), a correctly rounded division and then the nearest e4m3
- * value, ties to even. A NaN or infinity makes its block's scale NaN or infinite. Products of a row's
+ * scale = m / 448, q = e4m3(448 x / m), 448 x and the quotient each rounded to float32, ties to even.
+ * For 16-bit x that is the e4m3 value nearest to the exact quotient. A NaN or infinity makes its block's scale NaN or infinite. Products of a row's
  * and a weight's scale are float32: one that leaves its range is infinite or zero. */
 
 /* quantize_rows — x [n_tokens, hidden] f16, bf16 or f32 into q uint8 [rows, hidden] and scale f32

@@ -2,14 +2,16 @@
 // activations, 128 x 128 for weights.
 //
 // With m the largest magnitude of a block (at least 2^-96, so that a block of zeros has a finite
-// scale) the stored values are scale = m / 448 and q = e4m3(448 x / m): the correctly rounded
-// quotient, then the nearest e4m3 value, ties to even. 448 = 7 * 64, so 448 x is exact for 16-bit
-// x, and a quotient that lies midway between two e4m3 values comes out exactly midway; one product
+// scale) the stored values are scale = m / 448 and q = e4m3(448 x / m), 448 x and the quotient rounded
+// to float32, ties to even throughout. 448 = 7 * 64, so 448 x is exact for 16-bit x, a quotient
+// that lies midway between two e4m3 values comes out exactly midway, and any other is further
+// from there than its rounding: q is the value nearest to the exact quotient. Of float32 x a quotient within
+// two roundings (2^-23) of a midpoint may go to either neighbour. One product
 // with 1/m sends about one value in a thousand of bf16 data to the other neighbour.
 // A division per value is what the kernels would spend most of their time on (245 us for the
 // benchmark's gate and up projections, with two thirds of the issue slots busy). So the value is
 // bracketed by two products with 448/m, one a little small, one a little large (2^-21: more than
-// the four roundings between a product and the quotient can make). Rounding is monotone: where
+// the roundings between a product and the quotient can make, four of 2^-24, five of float32 x). Rounding is monotone: where
 // both give the same e4m3 value it is the quotient's, and only where they differ, around the
 // midpoints, the division decides.
 // A NaN makes its block's scale NaN, an infinity makes it infinite: the products that use the block

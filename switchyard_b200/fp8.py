@@ -93,7 +93,9 @@ def _no_grad(name, *tensors):
 def quantize_rows(x, plan=None):
     """Rows8 of x [N, H] (fp16, bf16 or fp32, H a multiple of 16). With a rows.SortPlan the rows come in
     expert order (as rows.permute_rows brings them), each token quantised once. With m the largest
-    magnitude of a block, at least 2^-96: scale = m / 448, q = e4m3(448 x / m), correctly rounded.
+    magnitude of a block, at least 2^-96: scale = m / 448, q = e4m3(448 x / m), the nearest value,
+    ties to even; of fp32 x, 448 x and the quotient are rounded to float32 first, so that one within 2^-23 of a
+    midpoint can go either way.
     A NaN or infinity in a block makes its scale NaN or infinite."""
     _no_grad("quantize_rows", x)
     x = x.contiguous()

@@ -100,6 +100,38 @@ def test_quantize_weight_is_exact(Q, E, N, K, halves, dtype):
     assert ((back - fine).abs() <= fine.abs() * (2.0 ** -4 + 2.0 ** -22) + 2.0 ** -10 * 6 / 448).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_quotients_next_to_a_midpoint(Q, dtype):
+    """448 x / m within the type's rounding of the middle between two e4m3 values. Of 16-bit values the result is the
+    e4m3 value nearest to the exact quotient (the oracle's division is in 64 bits, and no quotient of two 16-bit
+    numbers is nearer than 2^-20 to a midpoint that it is not). Of float32 values 448 x and the quotient are rounded
+    to float32 on the way, which may move a value across a midpoint: the result is within those two
+    roundings of half a step, not always the nearest."""
+    g = torch.Generator().manual_seed(5)
+    N = 256
+    m = (torch.rand(N, 1, generator=g) * 3 + 1).to(dtype)
+    if dtype is F32:
+        m[0] = 1.220261812210083
+    low = torch.randint(0, 0x7e, (N, 127), generator=g).to(torch.uint8)
+    mid = (low.view(torch.float8_e4m3fn).double() + (low + 1).view(torch.float8_e4m3fn).double()) / 2
+    x = (mid * m.double() / 448).to(dtype) * (1 - 2 * torch.randint(0, 2, (N, 127), generator=g)).to(dtype)
+    if dtype is F32:
+        x[0, 0] = 0.18521831929683685
+    x = torch.cat([m, x], 1)
+    for scale in (1.0, 2.0 ** -12, 2.0 ** 12) + ((2.0 ** -95, 2.0 ** 126 if dtype is F32 else 2.0 ** 100) if dtype is not HF else ()):
+        xs = x * scale
+        top = xs.abs().amax(1, keepdim=True)
+        exact = 448 * xs.double() / top.double()
+        want = rc.nearest8(exact)
+        if dtype is F32:
+            want, nearest = rc.nearest8((xs * (448 * 2.0 ** -16)) / (top * 2.0 ** -16)), want
+            assert (want != nearest).any()
+            assert ((want - exact).abs() <= (nearest - exact).abs() + 2.0 ** -22 * exact.abs()).all()
+        assert same(Q.quantize_rows(xs.to(DEV)).q.cpu().double(), want), scale
+        w = torch.cat([xs[:1], xs[1:2] * 0, xs[2:3] * 0], 0)[None]  # a block of one row's maximum
+        assert same(Q.quantize_weight(w.to(DEV)).q.cpu().double()[0, 0], want[0])
+
+
 def operands(counts, K, N, swiglu, seed):
     """Rows in expert order and weights, e4m3 values and scales on the CPU."""
     g = torch.Generator().manual_seed(seed)
