@@ -95,7 +95,7 @@ static_assert(G8_HELPERS * G8_REGS_FEW + 8 * G8_REGS_MANY <= (G8_HELPERS + 8) * 
 
 struct Gemm8Args {
   CUtensorMap wmap;   // [experts * halves * Nout, K] e4m3, box 128 k x WBOX
-  CUtensorMap xmap;   // [rows, K] e4m3, box 128 k x 128
+  CUtensorMap xmap;   // [rows, K] e4m3, box 128 k x 128 (not of the few-row tile)
   CUtensorMap xfew;   // the same, box 128 k x 32
   const float* xscale;  // [k blocks][rows]
   const float* wscale;  // [experts][halves * n blocks][k blocks]
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::v
     }
     fence_barrier_init();
     prefetch_tensormap(&args.wmap);
-    prefetch_tensormap(&args.xmap);
+    if (!FEW) prefetch_tensormap(&args.xmap);
     prefetch_tensormap(&args.xfew);
   }
   if (warp == 1) {
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(Shape8<TILE, std::is_same<T, __nv_fp8_e4m3>::v
         auto rows_of = [&](int c) { return min(max(tile.nvalid - c * S::XR, 0), S::XR); };
         auto boxes_of = [&](int n) { return (n + G8_XFEW - 1) / G8_XFEW; };  // of 32 rows
         const int mine = rows_of(cr), other = PAIR ? rows_of(cr ^ 1) : 0;
-        const bool few = mine < G8_XR;
+        const bool few = FEW || mine < G8_XR;
         const int x_boxes = few ? boxes_of(mine) : 1;
         const uint32_t bytes = WR * G8_BLOCK + (boxes_of(mine) + (PAIR ? boxes_of(other) : 0)) * (G8_XFEW * G8_BLOCK);  // of all CTAs
         const bool is_w = lane < S::W_BOXES, is_x = !is_w && lane - S::W_BOXES < x_boxes;
@@ -921,8 +921,10 @@ static int launch8(Gemm8Args a, const void* x, const void* w, cudaStream_t strea
   const uint64_t w_rows = (uint64_t)a.experts * (SWIGLU ? 2 : 1) * a.Nout;
   rc = tensor_map_2d(&a.wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, w_rows, (uint64_t)a.K, S::WBOX, G8_BLOCK);
   if (rc != SY_OK) return rc;
-  rc = tensor_map_2d(&a.xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XR, G8_BLOCK);
-  if (rc != SY_OK) return rc;
+  if (!S::FEW) {
+    rc = tensor_map_2d(&a.xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XR, G8_BLOCK);
+    if (rc != SY_OK) return rc;
+  }
   rc = tensor_map_2d(&a.xfew, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, (uint64_t)a.rows, (uint64_t)a.K, G8_XFEW, G8_BLOCK);
   if (rc != SY_OK) return rc;
   auto kern = gemm8_kernel<T, TILE, SWIGLU>;
