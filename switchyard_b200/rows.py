@@ -17,7 +17,6 @@ from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 
 class SortPlan(NamedTuple):
@@ -66,11 +65,26 @@ def _incoming(d):
     return d if d.data_ptr() % 16 == 0 else d.clone()
 
 
-def _once(backward):
-    """once_differentiable, entered only where a graph of the gradient is being recorded: its own guards are 5 us of
-    an 88 us pass forward and back."""
-    guarded = once_differentiable(backward)
-    return lambda ctx, *grads: guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+class _NoSecond(torch.autograd.Function):
+    """Hands its first tensors on, in a graph with all of them, and has no gradient."""
+
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tensors[:count]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("permute_rows and unpermute_rows have no second derivatives")
+
+
+def _last(grads, *inputs):
+    """The gradients, made from `inputs`. Where a graph of them is being recorded they are tied to those inputs: a
+    derivative of theirs is then refused, wherever it is asked for, and not left out of a sum (which is what
+    happens with torch's once_differentiable, whose error hangs on no input)."""
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)):
+        return grads
+    tied = iter(_NoSecond.apply(sum(g is not None for g in grads), *(g for g in grads if g is not None), *inputs))
+    return tuple(next(tied) if g is not None else None for g in grads)
 
 
 class _Permute(torch.autograd.Function):
@@ -80,10 +94,9 @@ class _Permute(torch.autograd.Function):
         return _ext().permute_rows(h, pos_of, offsets)
 
     @staticmethod
-    @_once
     def backward(ctx, dx):
         pos_of, = ctx.saved_tensors
-        return _ext().unpermute_rows(_incoming(dx), None, pos_of), None, None
+        return _last((_ext().unpermute_rows(_incoming(dx), None, pos_of), None, None), dx)
 
 
 class _Unpermute(torch.autograd.Function):
@@ -93,12 +106,11 @@ class _Unpermute(torch.autograd.Function):
         return _ext().unpermute_rows(y, w, pos_of)
 
     @staticmethod
-    @_once
     def backward(ctx, dout):
         y, w, offsets, pos_of = ctx.saved_tensors
         need_dy, need_dw = ctx.needs_input_grad[:2]
         dy, dw = _ext().unpermute_rows_grad(_incoming(dout), y, w, pos_of, offsets, need_dy, need_dw)
-        return dy, dw, None, None
+        return _last((dy, dw, None, None), dout, y, w)
 
 
 def permute_rows(h, plan):

@@ -130,6 +130,28 @@ def test_gradients_against_differences(R):
     assert abs(dot(dx, R.permute_rows(h + vh, p)) - dot(dx, R.permute_rows(h - vh, p)) - 2 * dot(dh, vh)) <= off
 
 
+def test_second_derivatives_are_refused_not_lost(R):
+    """dy depends on w and dw on y, whether or not the gradient that came in asks for one of its own: a gradient
+    of them has to end in an error, and not in the rest of a sum."""
+    idx, pos, p = setup(R, 6, 2, 4, 0, seed=14)
+    y, w = torch.randn(12, 64, device=DEV, requires_grad=True), torch.rand(6, 2, device=DEV, requires_grad=True)
+    dout = torch.ones(6, 64, device=DEV)
+    first, second = torch.autograd.grad(R.unpermute_rows(y, w, p), (y, w), dout, create_graph=True)
+    for loss, leaf in ((first.sum(), w), (second.sum(), y), ((first ** 2).sum() + w.sum(), w), (second.sum() + y.sum(), y)):
+        with pytest.raises(RuntimeError, match="second"):
+            torch.autograd.grad(loss, leaf, retain_graph=True)
+    d = dout.clone().requires_grad_()
+    h = torch.randn(6, 64, device=DEV, requires_grad=True)
+    dh, = torch.autograd.grad(R.permute_rows(h, p), h, torch.cat([d, d]), create_graph=True)
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(dh.sum() + d.sum(), d)
+    assert torch.equal(first.detach(), torch.autograd.grad(R.unpermute_rows(y, w, p), y, dout)[0])
+    one, = torch.autograd.grad(R.unpermute_rows(y, w.detach(), p), y, d, create_graph=True)  # w alone is a constant
+    assert torch.equal(one, first)
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(one.sum() + d.sum(), d)
+
+
 def test_the_order_of_the_sum_is_combines(R):
     """Without weights unpermute_rows gives combine's bits; with the weights applied to the rows
     first (float32 rows and products exact) the weighted sum's bits."""
