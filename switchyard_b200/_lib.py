@@ -12,6 +12,7 @@ from ctypes import c_char_p, c_int, c_size_t, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libswitchyard_b200.so")
+ROWS_PATH = os.path.join(HERE, "_rows_torch.so")
 
 SY_DTYPE_F16, SY_DTYPE_BF16, SY_DTYPE_F32 = 0, 1, 2
 SY_ERR_DEVICE = -3
@@ -97,6 +98,17 @@ def load():
             fn.restype, fn.argtypes = res, args
         _LIB = lib
     return _LIB
+
+
+def load_rows():
+    """The row operators' calls on torch tensors (csrc/rows_torch.cpp), over the loaded library."""
+    load()
+    if not os.path.exists(ROWS_PATH):
+        raise RuntimeError(f"{ROWS_PATH} is missing: build it with `python -m switchyard_b200.build`. "
+                           "switchyard_b200 has no CPU or PyTorch fallback.")
+    import torch  # noqa: F401  (its libraries first)
+    from . import _rows_torch
+    return _rows_torch
 
 
 def check(rc, what, lib=None):

@@ -1,18 +1,23 @@
-"""Builds the CUDA library in-tree with nvcc for sm_100a:
+"""Builds the CUDA library in-tree with nvcc for sm_100a, and the row operators' torch calls:
 
-    python -m switchyard_b200.build            # -> switchyard_b200/libswitchyard_b200.so
+    python -m switchyard_b200.build            # -> switchyard_b200/libswitchyard_b200.so, _rows_torch.so
 
-Plain nvcc, no torch headers: the library's boundary is a C ABI (include/switchyard_b200.h),
-so a build takes seconds and the product has no compile-time dependency on PyTorch."""
+The library: plain nvcc, no torch headers. Its boundary is a C ABI (include/switchyard_b200.h),
+so a build takes seconds and it has no compile-time dependency on PyTorch. The one file that has
+(csrc/rows_torch.cpp: autograd nodes over that C ABI) is an extension module of its own, no CUDA code in it."""
 
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libswitchyard_b200.so")
+ROWS = os.path.join(HERE, "_rows_torch.so")
+ROWS_SOURCE = os.path.join(CSRC, "rows_torch.cpp")
+HEADER = os.path.join(os.path.dirname(HERE), "include", "switchyard_b200.h")
 SOURCES = ["runtime.cu", "route.cu", "sort.cu", "combine.cu", "transport.cu", "gemm.cu", "ep.cu",
            "rows.cu", "quant8.cu", "gemm_fp8.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -26,18 +31,44 @@ def nvcc():
     return exe
 
 
+def _older(built, deps):
+    return not os.path.exists(built) or any(os.path.getmtime(d) > os.path.getmtime(built) for d in deps)
+
+
 def stale():
-    if not os.path.exists(LIB):
-        return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(os.path.dirname(HERE), "include", "switchyard_b200.h")]
-    return any(os.path.getmtime(d) > t for d in deps)
+    return _older(LIB, [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))] + [HEADER])
+
+
+def rows_stale():
+    return _older(ROWS, [ROWS_SOURCE, HEADER])
+
+
+def build_rows():
+    """Compile the row operators' extension module, linked to the library beside it."""
+    import torch
+    base = os.path.dirname(torch.__file__)
+    include = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include), ROWS_SOURCE,
+           "-o", ROWS, "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + HERE,
+           "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {os.path.basename(ROWS_SOURCE)}:\n{r.stdout}")
 
 
 def build(force=False, verbose=False):
-    """Compile every .cu of the package into one shared library. Returns its path."""
-    if not force and not stale():
-        return LIB
+    """Compile every .cu of the package into one shared library, and the extension module over it.
+    Returns the library's path."""
+    if force or stale():
+        build_library(verbose)
+    if force or rows_stale():
+        build_rows()
+    return LIB
+
+
+def build_library(verbose=False):
     objdir = os.path.join(HERE, "_obj")
     os.makedirs(objdir, exist_ok=True)
     procs = []
@@ -57,7 +88,6 @@ def build(force=False, verbose=False):
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}")
-    return LIB
 
 
 if __name__ == "__main__":

@@ -85,9 +85,11 @@ def refuse(name, *weights):
 
 
 def _no_grad(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    asks = _rows._ext().rows.asks(*tensors)
+    if asks == 2:
+        raise RuntimeError(f"{name} has no forward-mode derivative: unpack its dual inputs first")
+    if asks:
         raise RuntimeError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
-    _rows.refuse_tangents(name, *tensors)
 
 
 def quantize_rows(x, plan=None):

@@ -76,14 +76,6 @@ def _check_places(pos_of, offsets, dev, name):
     return pos_of.shape
 
 
-def _check_weights(w, rows, N, k, dev, name):
-    """Type code of the weights [N, k] of rows in dtype `rows`."""
-    if (w.dtype is not rows and w.dtype is not torch.float32) or w.shape != (N, k) or w.get_device() != dev or \
-            not w.is_contiguous():
-        raise RuntimeError(f"{name}: w must be contiguous [{N}, {k}], float32 or of the rows' dtype, on their CUDA device")
-    return _row_code(w, name)
-
-
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -137,6 +129,7 @@ class Ext:
 
     def __init__(self):
         self.lib = _lib.load()
+        self.rows = _lib.load_rows()  # the row operators: checks, allocation and autograd nodes in C++
         self._scratch = {}  # (device index, stream handle) -> Scratch of eager calls
 
     def scratch(self, device, stream):
@@ -335,55 +328,16 @@ class Ext:
 
     def permute_rows(self, h, pos_of, offsets):
         """x [N*k, H] with x[pos_of[t, j]] = h[t] (rows.permute_rows adds the gradient)."""
-        dev, code = _on_device(h, "permute_rows", "h"), _row_code(h, "permute_rows")
-        N, k = _check_places(pos_of, offsets, dev, "permute_rows")
-        if h.dim() != 2 or h.shape[0] != N:
-            raise RuntimeError(f"permute_rows: h must be [{N}, hidden], got {list(h.shape)}")
-        H = h.shape[1]
-        x = torch.empty((N * k, H), dtype=h.dtype, device=h.device)
-        with _Device(dev) as stream:
-            rc = self.lib.sy_permute_rows(h.data_ptr(), pos_of.data_ptr(), offsets.data_ptr(), N, k, offsets.numel() - 1, H,
-                                          code, x.data_ptr(), stream)
-        _lib.check(rc, "permute_rows")
-        return x
+        return self.rows.permute(h, pos_of, offsets)
 
     def unpermute_rows(self, y, w, pos_of):
         """out [N, H] = sum_j w[t, j] * y[pos_of[t, j]]; w None: all one (rows.unpermute_rows adds
         the gradients)."""
-        dev, code = _on_device(y, "unpermute_rows", "y"), _row_code(y, "unpermute_rows")
-        N, k = _check_places(pos_of, None, dev, "unpermute_rows")
-        if y.dim() != 2 or y.shape[0] != N * k:
-            raise RuntimeError(f"unpermute_rows: y must be [{N * k}, hidden], got {list(y.shape)}")
-        wcode = code if w is None else _check_weights(w, y.dtype, N, k, dev, "unpermute_rows")
-        H = y.shape[1]
-        out = torch.empty((N, H), dtype=y.dtype, device=y.device)
-        with _Device(dev) as stream:
-            rc = self.lib.sy_unpermute_rows(y.data_ptr(), _ptr(w), wcode, pos_of.data_ptr(), N, k, H, code, out.data_ptr(),
-                                            stream)
-        _lib.check(rc, "unpermute_rows")
-        return out
+        return self.rows.unpermute(y, w, pos_of)
 
     def unpermute_rows_grad(self, dout, y, w, pos_of, offsets, need_dy=True, need_dw=True):
         """(dy, dw) of unpermute_rows; what is not needed is None, and y may be None without dw."""
-        name = "unpermute_rows_grad"
-        dev, code = _on_device(dout, name, "dout"), _row_code(dout, name)
-        N, k = _check_places(pos_of, offsets, dev, name)
-        if dout.dim() != 2 or dout.shape[0] != N:
-            raise RuntimeError(f"{name}: dout must be [{N}, hidden], got {list(dout.shape)}")
-        H = dout.shape[1]
-        if y is not None and (y.dtype != dout.dtype or y.shape != (N * k, H) or _on_device(y, name, "y") != dev):
-            raise RuntimeError(f"{name}: y must be [{N * k}, {H}] in dout's dtype and on its device")
-        if need_dw and (y is None or w is None):
-            raise RuntimeError(f"{name}: the weights' gradient needs y and w")
-        wcode = code if w is None else _check_weights(w, dout.dtype, N, k, dev, name)
-        dy = torch.empty((N * k, H), dtype=dout.dtype, device=dout.device) if need_dy else None
-        dw = torch.empty_like(w) if need_dw else None
-        with _Device(dev) as stream:
-            rc = self.lib.sy_unpermute_rows_grad(dout.data_ptr(), _ptr(y), _ptr(w), wcode, pos_of.data_ptr(),
-                                                 offsets.data_ptr(), N, k, offsets.numel() - 1, H, code, _ptr(dy), _ptr(dw),
-                                                 stream)
-        _lib.check(rc, name)
-        return dy, dw
+        return self.rows.unpermute_grad(dout, y, w, pos_of, offsets, need_dy, need_dw)
 
     def quantize_rows(self, x, pos_of=None, offsets=None):
         """(q float8_e4m3fn [rows, H], scale float32 [ceil(H/128), rows]) of x [N, H]; with pos_of and

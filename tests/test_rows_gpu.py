@@ -152,6 +152,65 @@ def test_second_derivatives_are_refused_not_lost(R):
         torch.autograd.grad(one.sum() + d.sum(), d)
 
 
+def test_within_autograd(R):
+    """What autograd lets a user do with the nodes: ask for one of two gradients, run backward twice on a kept
+    graph and not on a freed one, recompute under checkpoint, keep saved tensors on the host, change a saved
+    plan (an error), and run from two threads."""
+    import threading
+
+    from torch.utils.checkpoint import checkpoint
+    idx, pos, p = setup(R, 21, 4, 16, 0, seed=15)
+    g = torch.Generator().manual_seed(4)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(BF).to(DEV)
+    h, w, d = rnd(21, 128).requires_grad_(), torch.rand(21, 4, generator=g).to(DEV).requires_grad_(), rnd(21, 128)
+    layer = lambda h, w: R.unpermute_rows(R.permute_rows(h, p) * 2, w, p)
+    out = layer(h, w)
+    dh, dw = torch.autograd.grad(out, (h, w), d, retain_graph=True)
+    for leaf, want in ((h, dh), (w, dw)):
+        assert torch.equal(torch.autograd.grad(out, leaf, d, retain_graph=True)[0], want)
+    out.backward(d)
+    assert torch.equal(h.grad, dh) and torch.equal(w.grad, dw)
+    with pytest.raises(RuntimeError, match="second time"):
+        out.backward(d)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(checkpoint(layer, h, w, use_reentrant=False), (h, w), d), (dh, dw)))
+    h.grad = w.grad = None
+    checkpoint(layer, h, w, use_reentrant=True).backward(d)
+    assert torch.equal(h.grad, dh) and torch.equal(w.grad, dw)
+    with torch.autograd.graph.save_on_cpu():
+        out = layer(h, w)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (h, w), d), (dh, dw)))
+    with torch.no_grad():
+        assert not layer(h, w).requires_grad
+    got = [None, None]
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = torch.autograd.grad(layer(h, w), (h, w), d)
+            torch.cuda.current_stream().synchronize()
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert all(torch.equal(a, b) for pair in got for a, b in zip(pair, (dh, dw)))
+    mine = R.SortPlan(*(t.clone() for t in p))
+    x = R.permute_rows(h, mine)
+    mine.pos_of.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        x.sum().backward()
+
+
+def test_functional_transforms_are_refused(R):
+    """Their wrappers have no memory of their own: an error, not a result without the transform."""
+    idx, pos, p = setup(R, 5, 2, 4, 0, seed=16)
+    h, y, w = torch.randn(5, 64, device=DEV), torch.randn(10, 64, device=DEV), torch.rand(5, 2, device=DEV)
+    calls = (lambda: torch.func.grad(lambda a: R.permute_rows(a, p).sum())(h), lambda: torch.func.grad(lambda a: R.unpermute_rows(y, a, p).sum())(w),
+             lambda: torch.func.jvp(lambda a: R.permute_rows(a, p), (h,), (h,)), lambda: torch.func.jvp(lambda a: R.unpermute_rows(a, w, p), (y,), (y,)),
+             lambda: torch.func.vmap(lambda a: R.permute_rows(a, p))(torch.stack([h, h])),
+             lambda: torch.func.vmap(lambda a: R.unpermute_rows(y, a, p))(torch.stack([w, w])))
+    for call in calls:
+        with pytest.raises(RuntimeError):
+            call()
+
+
 def test_the_order_of_the_sum_is_combines(R):
     """Without weights unpermute_rows gives combine's bits; with the weights applied to the rows
     first (float32 rows and products exact) the weighted sum's bits."""
