@@ -3,8 +3,6 @@ rounding bounds the tests hold the kernels to. Everything runs on the CPU."""
 
 import torch
 
-from oracle import moe_oracle as mo
-
 HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}  # eps / 2
 SMALLEST = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}  # half the least subnormal
 TINY = 2.0 ** -96
@@ -125,7 +123,3 @@ def swiglu_bound(acc, mag, K, N, dtype):
     ref = silu * u
     far = 1.1 * off[:, :N] * (u.abs() + off[:, N:]) + silu.abs() * off[:, N:] + 2.0 ** -20 * ref.abs()
     return ref, far + rounding(ref.abs() + far, dtype)
-
-
-def moe64(h, router_idx, w, gate_up, down):
-    return mo.experts_reference(h.double(), router_idx.long(), w.double(), gate_up.double(), down.double())
