@@ -428,6 +428,34 @@ def test_the_decoder_on_8_bit_experts(Q):
     assert d8.generate(prompts, 8, graph=True) == d8.generate(prompts, 8, graph=False)
 
 
+def test_the_decoder_s_8_bit_experts_are_its_own(Q):
+    """The 8-bit decoder against the same decoder on 16-bit experts: the dequantised ones, from which only the
+    rounding of two activations to e4m3 differs, and the originals. With Z what the logits move by when the
+    experts return nothing: an operand moves by at most 2^-4 of itself, so to first order an MoE output by at
+    most a 2^-4 part per rounded operand, and the logits by as much of Z: Z/8 for two, Z/4 for four, and
+    twice that for what lies beyond first order. Experts that return nothing or the
+    opposite, of another layer, or in another order move the logits by more than that."""
+    from switchyard_b200 import kernels, olmoe
+    c = olmoe.Config(vocab=211, hidden=256, intermediate=128, layers=3, heads=4, kv_heads=2, head_dim=64, experts=16, top_k=4,
+                     max_positions=128)
+    w = olmoe.random_weights(c, DEV, HF, seed=3, std=0.06)
+    toks = torch.randint(3, c.vocab, (3, 11), generator=torch.Generator().manual_seed(8)).to(DEV)
+    def logits(stacks, factor=1):
+        hook = lambda i, h: factor * kernels.moe_layer(h, w["layers"][i]["router"], *stacks[i], c.top_k, c.norm_topk_prob)
+        return olmoe.Decoder(c, w, hook).forward(toks).double()
+    plain = [(L["gate_up"], L["down"]) for L in w["layers"]]
+    rounded = [(Q.quantize_weight(gu, halves=2).dequantize(HF), Q.quantize_weight(dn).dequantize(HF)) for gu, dn in plain]
+    eight = [(L["gate_up"], L["down"]) for L in olmoe.quantize_experts(w)["layers"]]
+    got, ref, original = logits(eight), logits(rounded), logits(plain)
+    zero = (logits(rounded, 0) - ref).norm()
+    assert (got - ref).norm() <= zero / 4
+    assert (got - original).norm() <= zero / 2
+    shifted = [tuple(Q.Weight8(t.q.view(torch.uint8).roll(1, 0).view(t.q.dtype), t.scale.roll(1, 0), t.halves) for t in pair)
+               for pair in eight]
+    for wrong in (logits(eight, 0), logits(eight, -1), logits(eight[1:] + eight[:1]), logits(shifted)):
+        assert (wrong - ref).norm() > zero / 2
+
+
 def test_a_stack_quantised_as_one_is_not_taken_for_gate_and_up(Q):
     """Experts of width 200: the two layouts' scales have the same shape (four blocks of rows)."""
     from switchyard_b200 import kernels
