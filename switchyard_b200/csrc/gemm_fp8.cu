@@ -23,16 +23,16 @@
 //   token rows: an eighth of the promotion, 4 KB of token rows to fetch and read instead of 16, and results
 //   that go straight to memory, 32 columns of a row at a time. SwiGLU's up sums cross to the gates' warps
 //   through shared memory. 8-bit results take 256 weight rows, so that a tile has its 128 columns' maximum.
-//   (Token rows as M took 35.5 us for 8 tokens and 49.2 for 64, gate and up; this takes 31.5 and 44.2.)
+//   (Token rows as M took 35.5 us for 8 tokens and 49.2 for 64, gate and up; this takes 31.3 and 43.5.)
 //
 // What bounds it. Few rows per expert: the weights' way from HBM (64 tokens, 268 MB of gate and up: 44 us,
 // 6.1 TB/s), 3 us before the first ones arrive, and a last round of tiles, 3 to 4 us however few they are.
 // Many rows: a block of 256 columns over two CTAs takes 0.43 us where the MMAs alone take 0.27, with shared
 // memory busy for two thirds of it (by its bytes: 64 KB at 128 a clock), and the epilogues are a quarter
-// of a launch of 16 blocks a tile; and, run for seconds, the GPU's power: 8192 tokens take 292 us in a
-// burst, 341-350 us at 1.45 GHz and 990 W, of which the promotion's multiply-adds were 67 us. (The
-// library's 8-bit product of the same size, one scale per matrix, no experts, no SwiGLU, takes 246 us at
-// the same power.)
+// of a launch of 16 blocks a tile; and, run for seconds, the GPU's power: 8192 tokens take 303 us in a
+// burst of 2 ms, 344-361 us (from card to card) at 1.4 GHz and 990 W, of which the promotion's multiply-adds
+// were 67 us. (The library's 8-bit product of the same size, one scale per matrix, no experts, no SwiGLU,
+// takes 246 us at the same power.)
 #include <cuda.h>
 #include <cuda_fp8.h>
 
@@ -939,19 +939,28 @@ static int dispatch8(const Gemm8Args& a, int tile, const void* x, const void* w,
                            : launch8<T, G8_PAIR, SWIGLU>(a, x, w, s);
 }
 
-// Which tile a batch gets; the bits are the same. Measured on a B200 with the benchmark's layer (64 experts,
-// gate and up 2048 x 2048 with SwiGLU, down 2048 x 1024), us for the few / wide / pair tile:
-//   1 token     gate-up  9.6 / 13.5 / 14.2    down  6.9 /  8.6 /  9.6    8-bit results 11.8 / 14.3
-//   8 tokens            31.6 / 36.7 / 45.5         18.4 / 21.0 / 28.6                  33.7 / 38.1
-//   64 tokens           44.2 / 50.3 / 64.7         26.0 / 26.8 / 37.6                  47.7 / 51.5
-//   160 tokens          46.6 / 50.1                26.5 / 27.3                         47.1 / 50.9   (20 rows per expert)
-//   192 tokens          50.2 / 49.7                27.9 / 27.3                         47.6 / 50.9
-//   256 tokens          61.1 / 49.8                34.9 / 27.4                         52.2 / 50.7
-//   512 tokens           106 / 50.7 / 67.6         58.5 / 26.9 / 39.3
-//   1024 tokens                67.4 / 72.4                39.2 / 43.8
-//   4096 tokens                 167 /  168                 100 /  102
-//   8192 tokens                 305 /  303                 184 /  183   (1024 rows per expert)
+// Which tile a batch gets; the bits are the same. Measured on a B200 with the benchmark's layer (64 experts, top-8,
+// gate and up 2048 x 2048 with SwiGLU, down 2048 x 1024), us for the few / wide / pair tile: the fastest of five
+// graph replays of about 2 ms, 20 ms apart, over four weight sets (each larger than L2). Even routing, where
+// not called skewed (the most popular expert has 4.9 times the mean, the least 0.4):
+//   1 token     gate-up  9.5 / 13.4 / 14.0    down  6.6 /  8.8 /  8.7    8-bit results 11.5 / 13.7 / 14.6
+//   8 tokens            31.3 / 35.7 / 45.6         17.7 / 20.4 / 28.1                  32.7 / 36.8 / 48.1
+//   64 tokens           43.5 / 49.4 / 65.8         24.5 / 26.5 / 37.5                  45.9 / 50.2 / 67.9
+//   160 tokens          44.3 / 49.0 / 66.1         25.6 / 26.1 / 38.2                  45.8 / 50.1 / 68.2   (20 rows per expert)
+//      skewed           49.8 / 50.1 / 66.3         27.5 / 26.6 / 38.0                  48.9 / 50.8 / 68.4
+//   192 tokens          48.1 / 50.3 / 66.3         26.9 / 26.4 / 38.3                  44.6 / 51.0 / 68.3
+//      skewed           53.8 / 49.2 / 66.5         30.1 / 26.4 / 38.1                  51.0 / 50.4 / 68.6
+//   256 tokens          61.4 / 50.2 / 66.9         34.4 / 26.3 / 38.3                  52.3 / 50.6 / 68.8
+//   512 tokens                 51.5 / 69.7                26.9 / 39.7                         52.6 / 71.9
+//   1024 tokens                67.1 / 71.6                40.1 / 45.8                         67.2 / 72.4
+//   4096 tokens                 168 /  169                 101 /  103                          167 /  169
+//   6144 tokens                 240 /  241                 144 /  149                          237 /  239   (768)
+//      skewed                   241 /  235                 144 /  143                          237 /  234
+//   8192 tokens                 312 /  303                 187 /  185                          309 /  303
 // So: few up to 20 rows per expert (its 32 token rows are then seldom too few), pairs from 768, else wide.
+// At 20 rows per expert of other layers: 8 experts, gate and up 1024 x 1024, 6.2 / 7.5 (few rows win up to 50 rows per
+// expert, 6.7 / 7.5: the wide tiles do not fill the SMs); 16 experts 2048 x 2048, 15.7 / 16.0, skewed 17.7 / 15.9;
+// 60 experts 992 x 1040, 18.7 / 17.1; 128 experts 1024 x 1024, 27.0 / 27.0, skewed 31.7 / 27.3.
 static int choose_tile8(int rows, int experts) {
   return rows <= 20LL * experts ? G8_FEW : rows < 768LL * experts ? G8_WIDE : G8_PAIR;
 }

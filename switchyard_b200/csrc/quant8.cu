@@ -25,7 +25,7 @@ namespace sy {
 
 constexpr int Q8_BLOCK = 128;
 constexpr int Q8_THREADS = 256;         // weights
-constexpr int Q8_ROW_THREADS = 128;     // rows: small blocks that come and go (256: 36 us instead of 32 for 8192 tokens)
+constexpr int Q8_ROW_THREADS = 128;     // rows: small blocks that come and go (256: 36 us where this took 32, 8192 tokens)
 constexpr int Q8_LANES = Q8_BLOCK / 16;  // threads that share a row of a block, 16 columns each
 constexpr float Q8_TOP = 448.f;
 
@@ -118,7 +118,7 @@ template <typename T> __device__ __forceinline__ uint4 quantize16(const Sixteen<
 
 // A token's row is quantised once and stored at its k places in expert order (pos_of), or at its
 // own place (pos_of absent, k = 1). Bounded by the k stores: 8192 tokens, top-8, 2048 columns of bf16, 172 MB
-// in 32 us (5.3 TB/s), of which the scales' scattered four bytes are 3 us.
+// in 33 us (5.2 TB/s; 34 us a call of a loop), of which the scales' scattered four bytes are 3 us.
 // Scales are [blocks][rows]: what a tile of the product reads for one block is contiguous.
 template <typename T>
 __global__ void __launch_bounds__(Q8_ROW_THREADS, 10)
@@ -159,8 +159,8 @@ quantize_rows_kernel(const T* __restrict__ x, const int* __restrict__ pos_of, co
 }
 
 // One block of threads per 128 x 128 block of a weight matrix, which stays in registers between
-// the maximum and the division: every value crosses memory once (805 MB of bf16 in 139 us, 5.8 TB/s; issue
-// slots two thirds busy). 512 threads a block: 174 us, 128: 197.
+// the maximum and the division: every value crosses memory once (805 MB of bf16 in 140 us in a burst, 5.8 TB/s;
+// 151 a call of a loop; issue slots two thirds busy). 512 threads a block: 174 us, 128: 197.
 template <typename T>
 __global__ void __launch_bounds__(Q8_THREADS)
 quantize_weight_kernel(const T* __restrict__ w, int N, int K, uint8_t* __restrict__ q, float* __restrict__ scale) {

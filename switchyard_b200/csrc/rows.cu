@@ -27,8 +27,8 @@ static RowSplit row_split(int vecs) {
   return s;
 }
 
-// Bounded by the k stores per load: 8192 tokens, top-8, 2048 columns of bf16, 302 MB in 49.6 us (6.1 TB/s,
-// 0.93 of a copy's rate). Rows no choice was given (from offsets[n_experts] on, when the
+// Bounded by the k stores per load: 8192 tokens, top-8, 2048 columns of bf16, 302 MB in 50 us (6.0 TB/s,
+// 0.92 of a copy's rate). Rows no choice was given (from offsets[n_experts] on, when the
 // sort skipped invalid expert ids) are set to zero.
 __global__ void __launch_bounds__(ROWS_THREADS)
 permute_rows_kernel(const uint4* __restrict__ h, const int* __restrict__ pos_of, const int* __restrict__ rows_used,
@@ -52,7 +52,7 @@ permute_rows_kernel(const uint4* __restrict__ h, const int* __restrict__ pos_of,
 }
 
 // A token's rows are added in ascending sorted row, which is ascending expert id, ties by slot:
-// combine's order. float32 sum, one rounding. Bounded by reading the rows: the same 302 MB in 48.5 us.
+// combine's order. float32 sum, one rounding. Bounded by reading the rows: the same 302 MB in 46-48 us.
 template <typename T, typename W>
 __global__ void __launch_bounds__(ROWS_THREADS)
 unpermute_rows_kernel(const T* __restrict__ y, const W* __restrict__ w, const int* __restrict__ pos_of, int n_tokens,
@@ -100,7 +100,7 @@ unpermute_rows_kernel(const T* __restrict__ y, const W* __restrict__ w, const in
 
 // dy and dw in one pass over dout and y (either may be absent). The dot products are summed in
 // float32 over a thread's columns, then over the lanes, then over the warps of the token, always
-// in the same order. Bounded by HBM: 571 MB in 89.9 us (6.35 TB/s, 0.97 of a copy's rate); with all eight
+// in the same order. Bounded by HBM: 571 MB in 89.3 us (6.4 TB/s, 0.98 of a copy's rate); with all eight
 // rows' loads in flight and the places in registers (110 of them) two blocks of 256 fitted an SM: 135 us.
 template <typename T, typename W>
 __global__ void __launch_bounds__(ROWS_THREADS, 8)
