@@ -66,7 +66,7 @@ size_t sy_sort_scratch_bytes(int m, int n_experts);
 /* sort_by_expert — replaces `sort_by_expert` (moe_kernels.cu:142-157, kernels l.94-139 and the
  * torch cumsum between them). Stable counting sort of the flat choice list (i = token*top_k +
  * slot) by expert id, no atomics, same result every run.
- * idx int32 [m] (m = n_tokens*top_k, values in [0, n_experts)), w 16-bit [m] (or NULL: no weights,
+ * idx int32 [m] (m = n_tokens*top_k, at most 2^31 - 2^17, values in [0, n_experts)), w 16-bit [m] (or NULL: no weights,
  * wsorted is not written).
  * Outputs: counts int32 [n_experts]; offsets int32 [n_experts+1] (exclusive prefix);
  * token int32 [m] (= i / top_k of the choice in that sorted row); wsorted 16-bit [m];

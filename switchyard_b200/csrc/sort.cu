@@ -33,6 +33,10 @@ struct SortShape {
   int per_block;   // choices per block (multiple of 32 * SORT_WARPS)
 };
 
+// Most choices of a call: the last block's end, which may lie a round of threads per block beyond the last
+// choice, is still a 32-bit number (beyond it an index would come out negative).
+constexpr int SORT_MOST = 0x7ffe0000;
+
 static SortShape sort_shape(int m) {
   SortShape s;
   if (m <= SORT_SINGLE_MAX) {
@@ -44,7 +48,7 @@ static SortShape sort_shape(int m) {
   if (blocks > SORT_MAX_BLOCKS) blocks = SORT_MAX_BLOCKS;
   int per = (m + blocks - 1) / blocks;
   per = ((per + SORT_THREADS - 1) / SORT_THREADS) * SORT_THREADS;
-  s.blocks = (m + per - 1) / per;
+  s.blocks = (int)(((long long)m + per - 1) / per);
   s.per_block = per;
   return s;
 }
@@ -382,7 +386,7 @@ static int launch_sort(const int32_t* idx, const void* w, int m, int k, int E, i
 }  // namespace sy
 
 extern "C" size_t sy_sort_scratch_bytes(int m, int n_experts) {
-  if (m <= sy::SORT_SINGLE_MAX || n_experts <= 0) return 0;
+  if (m <= sy::SORT_SINGLE_MAX || m > sy::SORT_MOST || n_experts <= 0) return 0;
   return (size_t)sy::sort_shape(m).blocks * n_experts * sizeof(int);
 }
 
@@ -391,6 +395,7 @@ extern "C" int sy_sort_by_expert(const int32_t* idx, const void* w, int m, int t
                                  void* scratch, size_t scratch_bytes, void* stream) {
   using namespace sy;
   SY_REQUIRE(m >= 0 && top_k >= 1, "sort_by_expert: bad sizes (m=%d, k=%d)", m, top_k);
+  SY_REQUIRE(m <= SORT_MOST, "sort_by_expert: more than 2^31 - 2^17 choices");
   SY_REQUIRE(n_experts >= 1 && n_experts <= SORT_MAX_E, "sort_by_expert: at most %d experts (got %d)", SORT_MAX_E,
              n_experts);
   SY_REQUIRE(dtype == SY_DTYPE_F16 || dtype == SY_DTYPE_BF16, "sort_by_expert: dtype must be f16 or bf16");

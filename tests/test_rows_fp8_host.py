@@ -81,6 +81,14 @@ def test_quantisers_and_the_product_refuse(lib):
     refused(lib, lib.sy_sort_by_expert(P, P, 8, 2, 8, 0, P, P, P, None, P, None, 0, None), b"null")
 
 
+def test_the_sort_refuses_more_choices_than_it_can_count(lib):
+    """Just below 2^31 a block's end would pass 32 bits and an index come out negative."""
+    for m in (0x7fffffff, 0x7fff0000, 0x7ffe0001):
+        refused(lib, lib.sy_sort_by_expert(P, None, m, 1, 64, 0, P, P, P, None, P, P, 1 << 30, None), b"2^31")
+        assert lib.sy_sort_scratch_bytes(m, 64) == 0
+    assert lib.sy_sort_scratch_bytes(0x7ffe0000, 64) == 128 * 64 * 4
+
+
 def test_tensors_on_the_host_are_refused(lib):
     """There is no CPU path: every public call says so instead of computing something else."""
     from switchyard_b200 import fp8, rows
