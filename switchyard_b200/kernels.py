@@ -76,6 +76,12 @@ def _check_places(pos_of, offsets, dev, name):
     return pos_of.shape
 
 
+def _size(v):
+    """A size for the C ABI: past 32 bits the largest one, which the library refuses (ctypes would drop the upper
+    bits, and the call work on a part)."""
+    return min(int(v), 0x7fffffff)
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -245,10 +251,10 @@ class Ext:
         counts, offsets = ints[:E], ints[E:2 * E + 1]
         token, pos_of = ints[2 * E + 1:2 * E + 1 + M], ints[2 * E + 1 + M:]
         wsorted = torch.empty(M, dtype=w.dtype, device=dev) if w is not None else None
-        need = self.lib.sy_sort_scratch_bytes(M, int(E))
+        need = self.lib.sy_sort_scratch_bytes(_size(M), _size(E))
         scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         with _Device(dev) as stream:
-            _lib.check(self.lib.sy_sort_by_expert(_ptr(idx), _ptr(w), M, k, int(E), code, _ptr(counts), _ptr(offsets),
+            _lib.check(self.lib.sy_sort_by_expert(_ptr(idx), _ptr(w), _size(M), _size(k), _size(E), code, _ptr(counts), _ptr(offsets),
                                                   _ptr(token), _ptr(wsorted), _ptr(pos_of), _ptr(scratch), need, stream),
                        "sort_by_expert")
         return [counts, offsets, token, wsorted, pos_of]
@@ -357,8 +363,8 @@ class Ext:
         q = torch.empty((N * k, H), dtype=torch.float8_e4m3fn, device=x.device)
         scale = torch.empty(((H + 127) // 128, N * k), dtype=torch.float32, device=x.device)
         with _Device(dev) as stream:
-            rc = self.lib.sy_quantize_rows(x.data_ptr(), _ptr(pos_of), _ptr(offsets), N, k,
-                                           experts, H, code, q.data_ptr(), scale.data_ptr(), stream)
+            rc = self.lib.sy_quantize_rows(x.data_ptr(), _ptr(pos_of), _ptr(offsets), _size(N), _size(k),
+                                           _size(experts), _size(H), code, q.data_ptr(), scale.data_ptr(), stream)
         _lib.check(rc, "quantize_rows")
         return q, scale
 
@@ -372,8 +378,8 @@ class Ext:
         q = torch.empty(E, N, K, dtype=torch.float8_e4m3fn, device=w.device)
         scale = torch.empty(E, halves * ((N // halves + 127) // 128), (K + 127) // 128, dtype=torch.float32, device=w.device)
         with _Device(w.device) as stream:
-            _lib.check(self.lib.sy_quantize_weight(_ptr(w), E * halves, N // halves, K, code, _ptr(q), _ptr(scale), stream),
-                       "quantize_weight")
+            _lib.check(self.lib.sy_quantize_weight(_ptr(w), _size(E * halves), _size(N // halves), _size(K), code, _ptr(q),
+                                                   _ptr(scale), stream), "quantize_weight")
         return q, scale
 
     def grouped_gemm_fp8(self, x, x_scale, w, w_scale, offsets, swiglu, scale, dtype, tile=0):
@@ -406,7 +412,8 @@ class Ext:
         code = _lib.SY_DTYPE_F16 if dtype is torch.float16 else _lib.SY_DTYPE_BF16
         with _Device(dev) as stream:
             rc = self.lib.sy_grouped_gemm_fp8(x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
-                                              offsets.data_ptr(), E, rows, n_out, K, 1 if swiglu else 0, _ptr(scale),
+                                              offsets.data_ptr(), _size(E), _size(rows), _size(n_out), _size(K),
+                                              1 if swiglu else 0, _ptr(scale),
                                               C.data_ptr(), _ptr(c_scale), code, int(tile), stream)
         _lib.check(rc, name)
         return (C, c_scale) if out8 else C

@@ -476,6 +476,22 @@ def test_a_stack_quantised_as_one_is_not_taken_for_gate_and_up(Q):
     assert ((got - want).abs() <= product_bound(want, mag, 128, BF)[1] + 2.0 ** -22 * mag).all()
 
 
+def test_sizes_past_32_bits_are_refused(Q):
+    """Not taken for what their lower 32 bits say: 2^32 + 16 columns for 16."""
+    x = torch.empty(1, (1 << 32) + 16, dtype=BF, device=DEV)
+    with pytest.raises(RuntimeError, match="at most"):
+        Q.quantize_rows(x)
+    with pytest.raises(RuntimeError, match="at most"):
+        Q.quantize_weight(x[None])
+    del x
+    from switchyard_b200 import rows
+    p = rows.plan(torch.zeros(1, 1, dtype=torch.int32, device=DEV), 1)
+    h = torch.empty(1, (1 << 32) + 16, dtype=BF, device=DEV)
+    for call in (lambda: rows.permute_rows(h, p), lambda: rows.unpermute_rows(h, None, p)):
+        with pytest.raises(RuntimeError, match="at most"):
+            call()
+
+
 def test_streams_and_graphs(Q):
     """The same call on two streams at once and replayed from a graph, on new inputs."""
     offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([20, 0, 300], 256, 256, True, 9))

@@ -81,6 +81,19 @@ def test_quantisers_and_the_product_refuse(lib):
     refused(lib, lib.sy_sort_by_expert(P, P, 8, 2, 8, 0, P, P, P, None, P, None, 0, None), b"null")
 
 
+def test_sizes_past_32_bits_reach_the_library_as_the_largest(lib):
+    from switchyard_b200 import kernels
+    assert [kernels._size(v) for v in (0, 7, 0x7fffffff, 1 << 31, (1 << 32) + 16)] == [0, 7] + [0x7fffffff] * 3
+    most = kernels._size(1 << 32)
+    refused(lib, lib.sy_quantize_rows(P, None, None, most, 1, 0, 64, 1, P, P, None), b"2^31")
+    refused(lib, lib.sy_quantize_rows(P, None, None, 1, 1, 0, most, 1, P, P, None), b"at most")
+    refused(lib, lib.sy_quantize_weight(P, most, 8, 64, 1, P, P, None), b"matrices")
+    refused(lib, lib.sy_quantize_weight(P, 1, most, 64, 1, P, P, None), b"rows")
+    refused(lib, lib.sy_quantize_weight(P, 1, 8, most, 1, P, P, None), b"at most")
+    for sizes in ((most, 4, 64, 128), (8, most, 64, 128), (8, 4, most, 128), (8, 4, 64, most)):
+        assert lib.sy_grouped_gemm_fp8(P, P, P, P, P, *sizes, 0, None, P, None, 1, 0, None) == -1
+
+
 def test_the_sort_refuses_more_choices_than_it_can_count(lib):
     """Just below 2^31 a block's end would pass 32 bits and an index come out negative."""
     for m in (0x7fffffff, 0x7fff0000, 0x7ffe0001):
