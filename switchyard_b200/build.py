@@ -47,15 +47,18 @@ def build_rows():
     """Compile the row operators' extension module, linked to the library beside it."""
     import torch
     base = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
     include = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
-               sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    new = f"{ROWS}.{os.getpid()}"  # put in place whole: a process that loads it finds the old one or the new one
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include), ROWS_SOURCE,
-           "-o", ROWS, "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + HERE,
+           "-o", new, "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + HERE,
            "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {os.path.basename(ROWS_SOURCE)}:\n{r.stdout}")
+    os.replace(new, ROWS)
 
 
 def build(force=False, verbose=False):

@@ -11,7 +11,8 @@ Rows are fp16, bf16 or fp32 with a row of a multiple of 16 bytes, top_k is at mo
 not contiguous is copied first, one that is has to start on a 16-byte boundary; gradients may come in any
 form. Everything is enqueued on the current stream; nothing synchronises. There are no workspaces: what a captured graph
 keeps are the addresses of its tensors. Make the first call on a device outside a capture (it loads
-the library there). RuntimeError on any other argument, and for an input with a forward-mode
+the library there), and capture a backward pass with no eager graph of the same leaves alive (torch
+ties a leaf's gradient to the stream of the first). RuntimeError on any other argument, and for an input with a forward-mode
 tangent (the operators have gradients, no forward-mode and no second derivatives)."""
 
 from typing import NamedTuple
