@@ -492,6 +492,20 @@ def test_sizes_past_32_bits_are_refused(Q):
             call()
 
 
+def test_functional_transforms_are_refused(Q):
+    x, w = torch.randn(4, 128, device=DEV), torch.randn(2, 8, 128, device=DEV)
+    w8, offsets = Q.quantize_weight(w), torch.tensor([0, 2, 4], dtype=torch.int32, device=DEV)
+    x8 = Q.quantize_rows(x)
+    total = lambda r: (r.scale if isinstance(r, tuple) else r).sum()
+    calls = (lambda a: Q.quantize_rows(a), lambda a: Q.quantize_weight(a[None]),
+             lambda a: Q.grouped_gemm(x8, w8, offsets, scale=a[:, 0].bfloat16()))
+    for call in calls:
+        for transformed in (lambda: torch.func.grad(lambda a: total(call(a)))(x), lambda: torch.func.jvp(lambda a: total(call(a)), (x,), (x,)),
+                            lambda: torch.func.vmap(lambda a: total(call(a)))(torch.stack([x, x]))):
+            with pytest.raises(RuntimeError):
+                transformed()
+
+
 def test_streams_and_graphs(Q):
     """The same call on two streams at once and replayed from a graph, on new inputs."""
     offsets, xq, xs, wq, ws = (t.to(DEV) for t in operands([20, 0, 300], 256, 256, True, 9))
